@@ -18,10 +18,12 @@ DEBUG = os.environ.get("ATARAXOS_B200_DEBUG", "0") not in ("", "0")
 LIB_PATH = _LIB_DIR / ("libstratego_b200_debug.so" if DEBUG else "libstratego_b200.so")
 
 SB_OK, SB_E_ARG, SB_E_CUDA, SB_E_NOPOOL = 0, -1, -2, -3
-SB_DTYPE_F32, SB_DTYPE_BF16 = 0, 1
+SB_DTYPE_F32, SB_DTYPE_BF16, SB_DTYPE_F16 = 0, 1, 2
 SB_LAYOUT_DENSE_ALL, SB_LAYOUT_DENSE_LIVE, SB_LAYOUT_COMPACT = 0, 1, 2
 SB_POLICY_UNIFORM, SB_POLICY_GUMBEL = 0, 1
 SB_RULES_CUDA, SB_RULES_ISF = 0, 1
+SB_MASK_NONE, SB_MASK_U8, SB_MASK_BITS = 0, 1, 2
+SB_POLICY_MAX_ACTIONS, SB_POLICY_MAX_TOP, SB_POLICY_MAX_TEACHER = 65536, 32, 512
 SB_NOALLOC_MAX_ENVS = 262144
 SB_STATUS_BAD_SETUP = 1
 SB_STATUS_WAIT_TIMEOUT = 2
@@ -121,6 +123,28 @@ class SbHostIo(ctypes.Structure):
     ]
 
 
+class SbLogits(ctypes.Structure):
+    _fields_ = [("logits", vp), ("mask", vp), ("n_rows", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("mask_stride", ctypes.c_int64), ("n_actions", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("mask_kind", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
+class SbLogprobs(ctypes.Structure):
+    _fields_ = [("actions", vp), ("action_bytes", ctypes.c_int32), ("top", ctypes.c_int32), ("logprob", vp),
+                ("entropy", vp), ("row_stats", vp), ("top_action", vp), ("top_logprob", vp)]
+
+
+class SbLogprobsGrad(ctypes.Structure):
+    _fields_ = [("g_logprob", vp), ("g_entropy", vp), ("g_top", vp), ("g_logprob_stride", ctypes.c_int64),
+                ("g_entropy_stride", ctypes.c_int64), ("grad", vp)]
+
+
+class SbDistill(ctypes.Structure):
+    _fields_ = [("teacher_actions", vp), ("teacher_logits", vp), ("action_bytes", ctypes.c_int32),
+                ("teacher_dtype", ctypes.c_int32), ("listed", ctypes.c_int32), ("tail", ctypes.c_int32), ("loss", vp),
+                ("row_stats", vp)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "sb_abi_version": (ctypes.c_int, []),
@@ -153,6 +177,12 @@ _SIGS = {
     "sb_has_legal_movement": (ctypes.c_int, [ctypes.POINTER(SbState), vp, vp]),
     "sb_export_state": (ctypes.c_int, [ctypes.POINTER(SbState), ctypes.POINTER(SbExport), vp]),
     "sb_sum_move_number": (ctypes.c_int, [ctypes.POINTER(SbState), vp, vp]),
+    "sb_action_logprobs": (ctypes.c_int, [ctypes.POINTER(SbLogits), ctypes.POINTER(SbLogprobs), vp]),
+    "sb_action_logprobs_backward": (ctypes.c_int, [ctypes.POINTER(SbLogits), ctypes.POINTER(SbLogprobs),
+                                                   ctypes.POINTER(SbLogprobsGrad), vp]),
+    "sb_distill_loss": (ctypes.c_int, [ctypes.POINTER(SbLogits), ctypes.POINTER(SbDistill), vp]),
+    "sb_distill_loss_backward": (ctypes.c_int, [ctypes.POINTER(SbLogits), ctypes.POINTER(SbDistill), vp,
+                                                ctypes.c_int64, vp, vp]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -20,8 +20,8 @@ LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libstratego_b200.so"
 # the debug build: every kernel checks each game record's indices first (SB_DEBUG_BOUNDS)
 DEBUG_LIB_PATH = LIB_DIR / "libstratego_b200_debug.so"
-SOURCES = [CSRC / "sb_kernels.cu"]
-DEPS = SOURCES + [CSRC / "sb_device.cuh", INCLUDE / "stratego_b200.h"]
+SOURCES = [CSRC / "sb_kernels.cu", CSRC / "sb_policy.cu"]
+DEPS = SOURCES + [CSRC / "sb_device.cuh", CSRC / "sb_error.h", INCLUDE / "stratego_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

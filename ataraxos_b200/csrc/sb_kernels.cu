@@ -24,6 +24,7 @@
 #include <mutex>
 
 #include "sb_device.cuh"
+#include "sb_error.h"
 #include "stratego_b200.h"
 
 namespace sb {
@@ -1787,10 +1788,10 @@ __global__ void sum_move_kernel(const uint8_t* rec, int64_t n, int64_t* out) {
 static __device__ __align__(256) int64_t g_noalloc_actions[SB_NOALLOC_MAX_ENVS];
 
 namespace {
-
 thread_local char g_err[512] = "";
+}
 
-int fail(int code, const char* fmt, ...) {
+int sb::fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof g_err, fmt, ap);
@@ -1798,11 +1799,29 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-int cuda_fail(cudaError_t e, const char* what) {
+int sb::cuda_fail(cudaError_t e, const char* what) {
     return fail(SB_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+int sb::sm_count(int dev, int* out) {
+    static std::atomic<int> cache[64];
+    if (dev < 0 || dev >= 64) return fail(SB_E_ARG, "device index out of range");
+    int v = cache[dev].load(std::memory_order_relaxed);
+    if (!v) {
+        cudaError_t e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
+        cache[dev].store(v, std::memory_order_relaxed);
+    }
+    *out = v;
+    return SB_OK;
+}
+
+namespace {
+
+using sb::aligned;
+using sb::cuda_fail;
+using sb::fail;
+using sb::sm_count;
 
 int check_state(const sb_state* s) {
     if (!s) return fail(SB_E_ARG, "state is NULL");
@@ -1895,19 +1914,6 @@ int blocks_per_sm(const void* fn, int dev, int smem, int* out) {
     if (nb < 1) return fail(SB_E_CUDA, "kernel does not fit on an SM with %d bytes of shared memory", smem);
     if (g_nocc < CACHE_N) g_occ[g_nocc++] = OccEntry{fn, dev, smem, nb};
     *out = nb;
-    return SB_OK;
-}
-
-int sm_count(int dev, int* out) {
-    static std::atomic<int> cache[64];
-    if (dev < 0 || dev >= 64) return fail(SB_E_ARG, "device index out of range");
-    int v = cache[dev].load(std::memory_order_relaxed);
-    if (!v) {
-        cudaError_t e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
-        cache[dev].store(v, std::memory_order_relaxed);
-    }
-    *out = v;
     return SB_OK;
 }
 

@@ -34,6 +34,7 @@ from dataclasses import dataclass
 import torch
 
 from .buffer import NUM_ACTIONS, NUM_SQUARES, StrategoRolloutBuffer
+from .policy import action_logprobs
 from .selfplay import BatchedRolloutEngine, NetFn, _net_out
 
 R_PROPPLY = 160  # record byte offset of the cached proposal's ply (int32; -1 = no cached proposal)
@@ -92,6 +93,14 @@ class SearchResult:
     values: torch.Tensor       # [S] float32 value of every rollout, samples ordered (root, move, config)
     legal: torch.Tensor        # [S] int64 the first move of every rollout
     root_of: torch.Tensor      # [S] int64 the root of every rollout
+
+    def teacher(self, top: int = 32) -> tuple[torch.Tensor, torch.Tensor]:
+        """The search policy's ``top`` likeliest moves per root, as
+        :func:`ataraxos_b200.policy.distill_loss` takes its teacher: actions
+        ``[R,top]`` int64 (-1 past a root's last move) and their
+        log-probabilities ``[R,top]`` float32 (``tail=True`` counts the rest)."""
+        best = action_logprobs(torch.log(self.policy).float(), top=top)
+        return best.top_action, best.top_logprob
 
 
 class BatchedSearch:

@@ -25,6 +25,7 @@ import torch
 
 from . import _capi as C
 from .buffer import COMPACT_CHANNELS, MASK_BITS_BYTES, NUM_CHANNELS, NUM_SQUARES, StrategoRolloutBuffer, _POLICIES
+from .policy import ActionLogProbs, action_logprobs
 
 
 class TrajectoryBuffer:
@@ -104,6 +105,18 @@ class TrajectoryBuffer:
         self._run(n_plies, auto_reset)
         self.buf.ply += n_plies
         self.slot = (self.slot + n_plies) % self.T
+
+
+    def action_logprobs(self, logits: torch.Tensor, slots: slice = slice(None), *, top: int = 0,
+                        temperature: float = 1.0) -> ActionLogProbs:
+        """The ring's recorded actions under another policy: ``logits``
+        ``[S, n, 10000]``, a network's output for the observations of ``slots``
+        (default: all T), against those slots' legal masks.  ``logprob`` and
+        ``entropy`` are ``[S, n]`` (log-probability 0 in a slot whose game was over); see
+        :func:`ataraxos_b200.policy.action_logprobs`, gradients included."""
+        if self.mask is None:
+            raise RuntimeError("this ring keeps no legal masks (mask_format='none')")
+        return action_logprobs(logits, self.action[slots], self.mask[slots], top=top, temperature=temperature)
 
 
 class BeliefRollouts:

@@ -48,6 +48,7 @@ extern "C" {
 /* infostate element type and layout */
 #define SB_DTYPE_F32 0
 #define SB_DTYPE_BF16 1
+#define SB_DTYPE_F16 2         /* policy logits only */
 #define SB_LAYOUT_DENSE_ALL 0  /* [n,488,10,10]; every channel written */
 #define SB_LAYOUT_DENSE_LIVE 1 /* [n,488,10,10]; only channels 0-42, 456-487 written
                                   (43-455 must already be zero) */
@@ -337,6 +338,82 @@ int sb_export_state(const sb_state *s, const sb_export *out, void *stream);
 
 /* north-star: Σ move_number over envs into *out (current_step, cpp:301-303). */
 int sb_sum_move_number(const sb_state *s, int64_t *out, void *stream);
+
+/* ---- policy operators ------------------------------------------------------ */
+/* Rows of policy logits and the legal actions of each row, as the two
+ * operators below read them.  A masked-out logit is never looked at (it may
+ * hold anything); a row may have no legal action at all.  The policy of a row
+ * is softmax(logits / temperature) over its legal actions; sums and
+ * statistics are float32 whatever the logits' type. */
+#define SB_MASK_NONE 0         /* every action is legal */
+#define SB_MASK_U8 1           /* [n_rows, n_actions] bytes, non-zero = legal */
+#define SB_MASK_BITS 2         /* bit j of byte k = action 8k+j; bits past n_actions are ignored */
+#define SB_POLICY_MAX_ACTIONS 65536
+#define SB_POLICY_MAX_TOP 32   /* alternatives that sb_action_logprobs lists */
+#define SB_POLICY_MAX_TEACHER 512 /* listed teacher actions of sb_distill_loss */
+typedef struct sb_logits {
+    const void *logits;        /* element (r, a) at logits[r * row_stride + a] */
+    const uint8_t *mask;       /* row r at mask + r * mask_stride (NULL: SB_MASK_NONE) */
+    int64_t n_rows;
+    int64_t row_stride;        /* elements; 0 repeats one row */
+    int64_t mask_stride;       /* bytes; 0 repeats one row */
+    int32_t n_actions;         /* 1 .. SB_POLICY_MAX_ACTIONS */
+    int32_t dtype;             /* SB_DTYPE_F32 / BF16 / F16 */
+    int32_t mask_kind;         /* SB_MASK_* */
+    float temperature;         /* finite, > 0 */
+} sb_logits;
+
+/* Log-probabilities of given actions with entropy and top alternatives. */
+typedef struct sb_logprobs {
+    const void *actions;       /* [n_rows] signed integers, or NULL: none given */
+    int32_t action_bytes;      /* their size: 2, 4 or 8 */
+    int32_t top;               /* alternatives per row, 0 .. SB_POLICY_MAX_TOP */
+    float *logprob;            /* [n_rows]: 0 where the action is -1 (none), -inf where it is not
+                                  legal; may be NULL when actions is */
+    float *entropy;            /* [n_rows]: 0 for a row without a legal action */
+    float *row_stats;          /* [n_rows,2] kept for the backward pass (may be NULL) */
+    int64_t *top_action;       /* [n_rows,top] most likely first, ties to the lower action; -1
+                                  past the last action of non-zero probability */
+    float *top_logprob;        /* [n_rows,top], -inf there */
+} sb_logprobs;
+int sb_action_logprobs(const sb_logits *x, const sb_logprobs *out, void *stream);
+
+/* Gradient with respect to the logits; x, actions, top, entropy, row_stats
+ * and top_action as the forward call had or wrote them.  The gradients of the
+ * outputs may be NULL (zero).  Every element of grad is written (0 where the
+ * action is not legal). */
+typedef struct sb_logprobs_grad {
+    const float *g_logprob;    /* element r at [r * g_logprob_stride] (stride 0 or 1) */
+    const float *g_entropy;
+    const float *g_top;        /* [n_rows,top] */
+    int64_t g_logprob_stride;
+    int64_t g_entropy_stride;
+    void *grad;                /* [n_rows,n_actions] contiguous, the logits' type */
+} sb_logprobs_grad;
+int sb_action_logprobs_backward(const sb_logits *x, const sb_logprobs *fwd, const sb_logprobs_grad *g, void *stream);
+
+/* Divergence of the policy from a teacher that is given by its likeliest
+ * actions: per row sum q (log q - log p).  Entries whose action is negative
+ * or not legal, or whose teacher logit is -inf, are left out.
+ *   tail = 0: q = softmax(teacher logits / temperature) over the entries left;
+ *   tail = 1: the teacher logits are log-probabilities (at this temperature),
+ *     q = exp of them, and the actions not listed count as one more entry of
+ *     mass 1 - sum q against the policy's own mass on them. */
+typedef struct sb_distill {
+    const void *teacher_actions; /* [n_rows,listed] signed integers; one listed twice counts twice */
+    const void *teacher_logits;  /* [n_rows,listed] */
+    int32_t action_bytes;        /* 2, 4 or 8 */
+    int32_t teacher_dtype;       /* SB_DTYPE_* */
+    int32_t listed;              /* 1 .. SB_POLICY_MAX_TEACHER */
+    int32_t tail;                /* 0 or 1 */
+    float *loss;                 /* [n_rows] */
+    float *row_stats;            /* [n_rows,6] kept for the backward pass (may be NULL) */
+} sb_distill;
+int sb_distill_loss(const sb_logits *x, const sb_distill *d, void *stream);
+/* Gradient with respect to the student's logits; g_loss element r at
+ * [r * g_loss_stride] (stride 0 or 1), grad as in sb_logprobs_grad. */
+int sb_distill_loss_backward(const sb_logits *x, const sb_distill *d, const float *g_loss, int64_t g_loss_stride,
+                             void *grad, void *stream);
 
 #ifdef __cplusplus
 }

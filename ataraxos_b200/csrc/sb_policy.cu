@@ -7,8 +7,18 @@
 //   entropy H = log Z - (sum_L exp(d_a) d_a) / Z
 // One pass keeps (M, n, r, t): n entries equal to M, r = sum of exp(d) over
 // the others, t = sum of exp(d) d.  Holding the maximum's own 1 apart from r
-// keeps log Z = log n + log1p(r / n) exact to its last bits when one action
-// holds nearly all of the mass.
+// keeps log Z = log1p((n - 1) + r) exact to its last bits when one action
+// holds nearly all of the mass.  Sums are float32; exponentials are base 2
+// with log2(e) / T folded into the factor of x - M (the difference is taken
+// first, so large logits lose nothing).
+//
+// Layout of the work: a row belongs to one warp, or to the four warps of a
+// CTA where the bytes that a lane has to stream would make a long chain (more
+// than ROW_BYTES per row).  That rule looks at the shape and the types alone,
+// so a row's bits do not depend on the batch it comes in.  A legal mask is
+// staged in shared memory as one bit per action, and only the logits of set
+// bits are read: a position has some 30 legal moves of 10,000, so a row costs
+// its mask and 30 sectors instead of 20 or 40 KB.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,9 +33,14 @@
 namespace sb {
 namespace {
 
-constexpr int PT = 256;                   // threads of a row's CTA
+constexpr int WARPS = 4;                  // warps of a CTA: one row each, or one row together
+constexpr int ROW_BYTES = 4096;
 constexpr unsigned ALL = 0xffffffffu;
 constexpr float NEG_INF = -INFINITY;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int LIST = 1024;                // legal actions a warp gathers at once
+constexpr int BLOCK_WORDS = 8;            // mask words of a lane between two gathers
+constexpr int CHUNKS = 128;               // gradient chunks a warp lists at once
 
 struct Rows {
     const void* x;
@@ -43,11 +58,57 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-template <int MASK>
-__device__ __forceinline__ bool legal(const uint8_t* m, int a) {
-    if (MASK == SB_MASK_U8) return m[a] != 0;
-    if (MASK == SB_MASK_BITS) return (m[a >> 3] >> (a & 7)) & 1;
-    return true;
+__device__ __forceinline__ float exp2_(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(ALL, v, o);
+    return v;
+}
+
+// A chunk is 32 bytes of a row (one DRAM sector): 16 or 8 elements.
+template <typename T> struct Chunk {
+    static constexpr int E = 32 / sizeof(T);
+    uint32_t w[8];
+    __device__ __forceinline__ void load(const T* p) {
+        asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(p));
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    }
+    __device__ __forceinline__ void fill(uint32_t v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = v;
+    }
+    __device__ __forceinline__ float get(int e) const;
+    __device__ __forceinline__ void set(int e, float v);
+};
+template <> __device__ __forceinline__ float Chunk<float>::get(int e) const { return __uint_as_float(w[e]); }
+template <> __device__ __forceinline__ void Chunk<float>::set(int e, float v) { w[e] = __float_as_uint(v); }
+template <> __device__ __forceinline__ float Chunk<__nv_bfloat16>::get(int e) const {
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+}
+template <> __device__ __forceinline__ void Chunk<__nv_bfloat16>::set(int e, float v) {
+    const uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | b << 16 : (w[e >> 1] & 0xffff0000u) | b;
+}
+template <> __device__ __forceinline__ float Chunk<__half>::get(int e) const {
+    return __half2float(__ushort_as_half((unsigned short)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu)));
+}
+template <> __device__ __forceinline__ void Chunk<__half>::set(int e, float v) {
+    const uint32_t b = __half_as_ushort(__float2half_rn(v));
+    w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | b << 16 : (w[e >> 1] & 0xffff0000u) | b;
 }
 
 __device__ __forceinline__ int64_t load_index(const void* p, int bytes, int64_t i) {
@@ -62,42 +123,140 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i)
     return to_f(static_cast<const __half*>(p)[i]);
 }
 
+// ---- legal bits in shared memory -------------------------------------------
+
+// Bit a + P of `w` is 1 where action a is legal; words before and after the
+// row are 0, so a field that reaches past either end reads zeros.
+struct Bits {
+    uint32_t* w;
+    int p;
+    __device__ __forceinline__ bool test(int a) const { return (w[(a + p) >> 5] >> ((a + p) & 31)) & 1; }
+    // `len` <= 16 bits of the actions from a on (a >= -16)
+    __device__ __forceinline__ uint32_t field(int a, int len) const {
+        const int b = a + p;
+        return __funnelshift_r(w[b >> 5], w[(b >> 5) + 1], b & 31) & ((1u << len) - 1u);
+    }
+};
+
+// Bytes of a staged row: the bits, 32 of lead (16 to align a bit-packed row's
+// chunks, 16 of zeros) and zeros past the end.
+__host__ __device__ constexpr int bits_bytes(int a) { return ((a + 7) / 8 + 32 + 48 + 15) / 16 * 16; }
+
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t v) {  // bit i: byte i of v is not 0
+    const uint32_t t = (((v & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v) & 0x80808080u;
+    return ((t >> 7) * 0x01020408u) >> 24 & 15u;
+}
+
+// Stage one row's mask with G threads (tid 0..G-1; the caller synchronises).
+template <int MASK, int G>
+__device__ __forceinline__ Bits stage(uint8_t* sh, const uint8_t* m, int a, int tid) {
+    const int h = (int)(-(intptr_t)m & 15), off = (16 - h) & 15;
+    if (MASK == SB_MASK_BITS) {
+        // Row byte i goes to sh[16 + off + i], so that the 16-byte chunks of
+        // the row in memory stay 16-byte chunks here.  The row's last byte is
+        // always handled as a tail byte: its bits past the last action drop.
+        const int len = (a + 7) >> 3, nb = len - h > 0 ? (len - h - 1) >> 4 : 0;
+        uint4* s4 = reinterpret_cast<uint4*>(sh + 16 + off + h);
+        const uint4* g4 = reinterpret_cast<const uint4*>(m + h);
+#pragma unroll 3
+        for (int j = tid; j < nb; j += G) s4[j] = __ldg(g4 + j);
+        const uint8_t last = (uint8_t)(0xffu >> (-a & 7));
+        for (int q = tid; q < 64; q += G) {  // 32 lead bytes (head included), then 32 tail bytes
+            const int i = q < 32 ? q - 16 - off : h + 16 * nb + q - 32;
+            if (q < 32 && i >= h) continue;
+            uint8_t v = 0;
+            if (i >= 0 && i < len) v = i == len - 1 ? m[i] & last : m[i];
+            sh[16 + off + i] = v;
+        }
+        return {reinterpret_cast<uint32_t*>(sh), 8 * (16 + off)};
+    }
+    // One byte per action: 16 of them make one halfword.
+    uint16_t* s2 = reinterpret_cast<uint16_t*>(sh);
+    const int lead = 2 + (h > 0), nb = a > h ? (a - h) >> 4 : 0;
+    const uint4* g4 = reinterpret_cast<const uint4*>(m + h);
+#pragma unroll 5
+    for (int j = tid; j < nb; j += G) {
+        const uint4 v = __ldg(g4 + j);
+        uint32_t b = 0;
+        if (v.x | v.y | v.z | v.w)
+            b = nonzero_bytes(v.x) | nonzero_bytes(v.y) << 4 | nonzero_bytes(v.z) << 8 | nonzero_bytes(v.w) << 12;
+        s2[lead + j] = (uint16_t)b;
+    }
+    if (tid < 32) {
+        const int i = tid < 16 ? tid - off : h + 16 * nb + tid - 16;
+        const bool on = tid < 16 ? (i >= 0 && i < h && i < a) : i < a;
+        const uint32_t b = __ballot_sync(ALL, on && m[on ? i : 0] != 0);
+        if (tid < 2) s2[tid] = 0;
+        if (tid == 2 && h > 0) s2[2] = (uint16_t)(b & 0xffffu);
+        if (tid >= 8 && tid < 16) s2[lead + nb + tid - 8] = tid == 8 ? (uint16_t)(b >> 16) : 0;
+    }
+    return {reinterpret_cast<uint32_t*>(sh), 32 + off};
+}
+
+// ---- running sums ------------------------------------------------------------
+
+// M is the same in all lanes of a warp; n, r and t are the lane's own shares.
+// t is in units of log2(e): sum of exp(d) d log2(e).
 struct Sum {
     float m, n, r, t;
 };
-__device__ __forceinline__ Sum empty_sum() { return {NEG_INF, 0.f, 0.f, 0.f}; }
 
-__device__ __forceinline__ Sum merge(Sum a, Sum b, float inv_t) {
-    if (b.m > a.m) {
-        const Sum c = a;
-        a = b;
-        b = c;
+// Take up a tile of N logits per lane (-inf where there is none).  A NaN
+// reaches r; +inf stays the maximum; both make the row NaN at the end.
+template <int N, bool ENT>
+__device__ __forceinline__ void take(Sum& s, const float (&x)[N], float c) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+    m = warp_max(fmaxf(m, NEG_INF));
+    if (m > s.m) {
+        const float d = (s.m - m) * c, f = exp2_(d), w = s.r + s.n;
+        if (ENT) s.t = f * (s.t + w * fmaxf(d, -1e4f));
+        s.r = f * w;
+        s.n = 0.f;
+        s.m = m;
     }
-    if (a.m == b.m) return {a.m, a.n + b.n, a.r + b.r, a.t + b.t};
-    const float d = (b.m - a.m) * inv_t, e = expf(d), w = b.n + b.r;
-    a.r += e > 0.f ? e * w : (w != w ? w : 0.f);
-    if (e > 0.f) a.t += e * (b.t + w * d);
+    const float ref = s.m == NEG_INF ? 0.f : s.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = (x[i] - ref) * c, e = exp2_(d);
+        if (x[i] == ref) s.n += 1.f;
+        else s.r += e;
+        if (ENT) s.t = fmaf(e, fmaxf(d, -1e4f), s.t);
+    }
+}
+
+__device__ __forceinline__ Sum no_sum() { return {NEG_INF, 0.f, 0.f, 0.f}; }
+
+// Two sums as one; both in full (all lanes' shares joined).
+__device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
+    if (b.m > a.m) {
+        const Sum q = a;
+        a = b;
+        b = q;
+    }
+    const bool eq = a.m == b.m;
+    const float d = eq ? 0.f : (b.m - a.m) * c, f = exp2_(d), w = b.r + b.n;
+    a.t += f * (b.t + (eq ? 0.f : w * fmaxf(d, -1e4f)));
+    a.r += eq ? b.r : f * w;
+    a.n += eq ? b.n : 0.f;
     return a;
 }
 
-__device__ __forceinline__ Sum one(float x) {
-    if (x != x || x == INFINITY) return {NEG_INF, 0.f, NAN, 0.f};
-    return {x, x == NEG_INF ? 0.f : 1.f, 0.f, 0.f};
-}
-
-__device__ __forceinline__ float log_z(Sum s) { return logf(s.n) + log1pf(s.r / s.n); }
-
-__device__ Sum block_merge(Sum s, float inv_t, Sum* sh) {
-    for (int o = 16; o; o >>= 1) {
-        Sum b = {__shfl_xor_sync(ALL, s.m, o), __shfl_xor_sync(ALL, s.n, o), __shfl_xor_sync(ALL, s.r, o),
-                 __shfl_xor_sync(ALL, s.t, o)};
-        s = merge(s, b, inv_t);
+// The sum of a whole row in every thread: over the warp's lanes, then over
+// the row's warps by way of shared memory.
+template <int W>
+__device__ __forceinline__ Sum whole(Sum s, float c, Sum* sh) {
+    s.n = warp_sum(s.n);
+    s.r = warp_sum(s.r);
+    s.t = warp_sum(s.t);
+    if (W > 1) {
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = sh[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) s = join(s, sh[w], c);
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = sh[0];
-    for (int w = 1; w < PT / 32; ++w) s = merge(s, sh[w], inv_t);
     return s;
 }
 
@@ -105,251 +264,550 @@ __device__ Sum block_merge(Sum s, float inv_t, Sum* sh) {
 // row without an action of non-zero probability (every p is then 0) and NaN
 // for a row that holds a legal NaN or +inf.
 __device__ __forceinline__ float2 stats_of(Sum s) {
-    if (s.r != s.r) return make_float2(0.f, NAN);
+    if (s.r != s.r || s.m == INFINITY) return make_float2(0.f, NAN);
     if (s.m == NEG_INF) return make_float2(0.f, INFINITY);
-    return make_float2(s.m, log_z(s));
+    return make_float2(s.m, log1pf((s.n - 1.f) + s.r));
 }
 
-template <typename T, int MASK>
-__global__ void __launch_bounds__(PT) logprobs_kernel(Rows R, sb_logprobs o) {
-    __shared__ Sum sh[PT / 32];
-    __shared__ float best_x[PT / 32];
-    __shared__ int best_a[PT / 32];
-    for (int64_t row = blockIdx.x; row < R.n; row += gridDim.x) {
-        const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        const uint8_t* m = R.mask + row * R.mask_stride;
-        Sum s = empty_sum();
-        for (int a = threadIdx.x; a < R.a; a += PT)
-            if (legal<MASK>(m, a)) s = merge(s, one(to_f(x[a])), R.inv_t);
-        s = block_merge(s, R.inv_t, sh);
-        const float2 st = stats_of(s);
-        if (threadIdx.x == 0) {
-            if (o.logprob) {
-                const int64_t act = load_index(o.actions, o.action_bytes, row);
-                float lp = NEG_INF;
-                if (act == -1) lp = 0.f;
-                else if (act >= 0 && act < R.a && legal<MASK>(m, (int)act)) lp = (to_f(x[act]) - st.x) * R.inv_t - st.y;
-                o.logprob[row] = lp;
+// ---- the likeliest actions ------------------------------------------------------
+
+// A warp's best `k` entries in descending order, one per lane; ties go to the
+// lower action.
+struct Top {
+    float x, bar_x;  // this lane's entry; the k-th one
+    int a, bar_a, k;
+    __device__ __forceinline__ void init(int n) {
+        x = bar_x = NEG_INF;
+        a = bar_a = 0x7fffffff;
+        k = n;
+    }
+    __device__ __forceinline__ bool wants(float v, int b) const {
+        return v > bar_x || (v == bar_x && b < bar_a && v > NEG_INF);
+    }
+    __device__ __noinline__ void offer(float v, int b) {  // one candidate per lane (-inf: none)
+        unsigned c = __ballot_sync(ALL, wants(v, b));
+        while (c) {
+            const int src = __ffs(c) - 1;
+            const float cx = __shfl_sync(ALL, v, src);
+            const int ca = __shfl_sync(ALL, b, src);
+            const int at = __popc(__ballot_sync(ALL, x > cx || (x == cx && a < ca)));
+            const float ux = __shfl_up_sync(ALL, x, 1);
+            const int ua = __shfl_up_sync(ALL, a, 1);
+            const int lane = threadIdx.x & 31;
+            if (lane >= at) {
+                x = lane == at ? cx : ux;
+                a = lane == at ? ca : ua;
             }
-            o.entropy[row] = st.y == INFINITY ? 0.f : st.y - s.t / (s.n + s.r);
-            if (o.row_stats) {
-                o.row_stats[2 * row] = st.x;
-                o.row_stats[2 * row + 1] = st.y;
-            }
+            bar_x = __shfl_sync(ALL, x, k - 1);
+            bar_a = __shfl_sync(ALL, a, k - 1);
+            c &= c - 1;
+            c &= __ballot_sync(ALL, wants(v, b));
         }
-        float last_x = INFINITY;
-        int last_a = -1;
-        for (int k = 0; k < o.top; ++k) {
-            float bx = NEG_INF;
-            int ba = -1;
-            for (int a = threadIdx.x; a < R.a; a += PT) {
-                if (!legal<MASK>(m, a)) continue;
-                const float v = to_f(x[a]);
-                if ((v < last_x || (v == last_x && a > last_a)) && v > bx) {
-                    bx = v;
-                    ba = a;
+    }
+};
+
+// ---- one pass over a row ------------------------------------------------------------
+
+// The legal logits of this warp's part of a row: `w` of W parts.  `skip`
+// holds bits (laid out like the mask's) of actions to leave out, or NULL.
+template <typename T, int W, bool ENT, bool TOP>
+__device__ __forceinline__ void pass_masked(Sum& s, Top& top, const T* x, Bits bits, const uint32_t* skip, int a, float c,
+                                            uint16_t* list, int part) {
+    const int lane = threadIdx.x & 31;
+    const int words = (bits.p + a + 31) >> 5;
+    for (int w0 = part * 32; w0 < words; w0 += 32 * BLOCK_WORDS * W) {
+        // lane's words: w0 + lane + k * 32 * W
+        uint32_t w[BLOCK_WORDS];
+        int count = 0;
+#pragma unroll
+        for (int k = 0; k < BLOCK_WORDS; ++k) {
+            const int i = w0 + lane + k * 32 * W;
+            w[k] = i < words ? bits.w[i] & (skip ? ~skip[i] : ALL) : 0u;
+            count += __popc(w[k]);
+        }
+        int at = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(ALL, at, o);
+            if (lane >= o) at += v;
+        }
+        const int total = __shfl_sync(ALL, at, 31);
+        if (total <= LIST) {
+            at -= count;
+#pragma unroll
+            for (int k = 0; k < BLOCK_WORDS; ++k) {
+                const int base = (w0 + lane + k * 32 * W) * 32 - bits.p;
+                while (w[k]) {
+                    list[at++] = (uint16_t)(base + __ffs(w[k]) - 1);
+                    w[k] &= w[k] - 1;
                 }
             }
-            for (int q = 16; q; q >>= 1) {
-                const float vx = __shfl_xor_sync(ALL, bx, q);
-                const int va = __shfl_xor_sync(ALL, ba, q);
-                if (vx > bx || (vx == bx && va < ba)) {
-                    bx = vx;
-                    ba = va;
+            __syncwarp();
+            for (int i = 0; i < total; i += 128) {
+                float v[4];
+                int b[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int n = i + q * 32 + lane;
+                    b[q] = n < total ? list[n] : 0;
+                    v[q] = n < total ? to_f(x[b[q]]) : NEG_INF;
+                }
+                take<4, ENT>(s, v, c);
+                if (TOP)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) top.offer(v[q], b[q]);
+            }
+            __syncwarp();
+        } else {
+            // too many for the list: every word's 32 actions in turn, a lane each
+#pragma unroll
+            for (int k = 0; k < BLOCK_WORDS; ++k) {
+                const int base = (w0 + k * 32 * W) * 32 - bits.p + lane;
+                if (!__any_sync(ALL, w[k])) continue;
+                for (int j = 0; j < 32; j += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const uint32_t m = __shfl_sync(ALL, w[k], j + q);
+                        v[q] = (m >> lane) & 1 ? to_f(x[base + 32 * (j + q)]) : NEG_INF;
+                    }
+                    take<8, ENT>(s, v, c);
+                    if (TOP)
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) top.offer(v[q], base + 32 * (j + q));
                 }
             }
-            __syncthreads();
-            if ((threadIdx.x & 31) == 0) {
-                best_x[threadIdx.x >> 5] = bx;
-                best_a[threadIdx.x >> 5] = ba;
-            }
-            __syncthreads();
-            bx = best_x[0];
-            ba = best_a[0];
-            for (int w = 1; w < PT / 32; ++w)
-                if (best_x[w] > bx || (best_x[w] == bx && best_a[w] < ba)) {
-                    bx = best_x[w];
-                    ba = best_a[w];
-                }
-            if (threadIdx.x == 0) {
-                o.top_action[row * o.top + k] = ba;
-                o.top_logprob[row * o.top + k] = st.y != st.y ? NAN : ba < 0 ? NEG_INF : (bx - st.x) * R.inv_t - st.y;
-            }
-            last_x = bx;
-            last_a = ba < 0 ? 0x7fffffff : ba;
         }
     }
 }
 
-// Gradient of one row: p (c0 + c1 log p) off the listed actions, and
-// p (l0 + c1 log p) + (the sum of its entries' shares) on them.
+// The same without a mask: 32-byte chunks of the row at their alignment in
+// memory, the ends that do not fill one by single loads.
+template <typename T, int W, bool ENT, bool TOP>
+__device__ __forceinline__ void pass_all(Sum& s, Top& top, const T* x, const Bits* skip, int a, float c, int part) {
+    constexpr int E = Chunk<T>::E, U = 32 / E;
+    const int lane = threadIdx.x & 31;
+    const int head = min(a, (int)((-(intptr_t)x & 31) / sizeof(T))), chunks = (a - head) / E;
+    if (part == 0) {  // the ends: fewer than two chunks, one element a lane
+        const int tail = head + chunks * E;
+        const int b = lane < head ? lane : tail + lane - head;
+        const bool on = b < a && !(skip && skip->test(b));
+        float v[1] = {on ? to_f(x[b]) : NEG_INF};
+        take<1, ENT>(s, v, c);
+        if (TOP) top.offer(v[0], b);
+    }
+    const T* body = x + head;
+    for (int c0 = part * 32 * U; c0 < chunks; c0 += 32 * U * W) {
+        Chunk<T> q[U];
+        float v[32];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = c0 + u * 32 + lane;
+            if (i < chunks) q[u].load(body + i * E);
+        }
+        float m = NEG_INF;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = c0 + u * 32 + lane;
+            const uint32_t out = i >= chunks ? ALL : skip ? skip->field(head + i * E, E) : 0u;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[u * E + e] = (out >> e) & 1 ? NEG_INF : q[u].get(e);
+                m = fmaxf(m, v[u * E + e]);
+            }
+        }
+        take<32, ENT>(s, v, c);
+        if (TOP && __any_sync(ALL, m >= top.bar_x)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = c0 + u * 32 + lane;
+                for (int e = 0; e < E; ++e)  // read again from cache: this is the rare path
+                    top.offer(i < chunks ? to_f(body[i * E + e]) : NEG_INF, head + i * E + e);
+            }
+        }
+    }
+}
+
+// ---- forward: given actions, entropy, top alternatives -----------------------------
+
+template <int MASK, int W>
+__host__ __device__ constexpr int list_bytes() { return MASK == SB_MASK_NONE ? 0 : 2 * LIST; }
+
+template <typename T, int MASK, int W, bool TOP>
+__global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprobs o) {
+    extern __shared__ uint4 dyn[];
+    __shared__ Sum sums[WARPS];
+    __shared__ float top_x[WARPS][32];
+    __shared__ int top_a[WARPS][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
+    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
+    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
+    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
+    const float c = R.inv_t * LOG2E;
+    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
+    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
+        const T* x = static_cast<const T*>(R.x) + row * R.stride;
+        int64_t act = -1;
+        float xa = 0.f;
+        if (o.actions) {
+            act = load_index(o.actions, o.action_bytes, row);
+            if (act >= 0 && act < R.a) xa = to_f(x[act]);
+        }
+        Sum s = no_sum();
+        Top top;
+        top.init(TOP ? o.top : 1);
+        bool legal = act >= 0 && act < R.a;
+        if (MASK == SB_MASK_NONE) {
+            pass_all<T, W, true, TOP>(s, top, x, nullptr, R.a, c, W == 1 ? 0 : warp);
+        } else {
+            const Bits bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            if (W == 1) __syncwarp();
+            else __syncthreads();
+            legal = legal && bits.test((int)act);
+            pass_masked<T, W, true, TOP>(s, top, x, bits, nullptr, R.a, c, list, W == 1 ? 0 : warp);
+        }
+        if (TOP && W > 1) {
+            top_x[warp][lane] = top.x;
+            top_a[warp][lane] = top.a;
+        }
+        s = whole<W>(s, c, sums);
+        const float2 st = stats_of(s);
+        if (W == 1 || warp == 0) {
+            if (lane == 0) {
+                if (o.logprob) o.logprob[row] = act == -1 ? 0.f : legal ? (xa - st.x) * R.inv_t - st.y : NEG_INF;
+                o.entropy[row] = st.y == INFINITY ? 0.f : st.y - LN2 * s.t / (s.n + s.r);
+                if (o.row_stats) *reinterpret_cast<float2*>(o.row_stats + 2 * row) = st;
+            }
+            if (TOP) {
+                if (W > 1)
+#pragma unroll
+                    for (int w = 1; w < W; ++w) top.offer(lane < o.top ? top_x[w][lane] : NEG_INF, top_a[w][lane]);
+                if (lane < o.top) {
+                    const bool some = top.x > NEG_INF;
+                    o.top_action[row * o.top + lane] = some ? top.a : -1;
+                    o.top_logprob[row * o.top + lane] =
+                        st.y != st.y ? NAN : some ? (top.x - st.x) * R.inv_t - st.y : NEG_INF;
+                }
+            }
+        }
+        if (W > 1) __syncthreads();
+        else __syncwarp();
+    }
+}
+
+// ---- gradient rows ---------------------------------------------------------------------
+
+// Gradient of a row: p (c0 + c1 log p) / T off the listed actions, and
+// (p (l0 + c1 log p) + the sum of its entries' shares) / T on them.
 struct RowGrad {
     float m, logz, c0, c1, l0;
 };
 
-template <typename T, int MASK>
-__device__ void write_grad(const Rows& R, const T* x, const uint8_t* m, T* g, RowGrad c, int listed, const int* idx,
-                           const float* add) {
-    for (int a = threadIdx.x; a < R.a; a += PT) {
-        float v = 0.f;
-        if (legal<MASK>(m, a)) {
-            const float lp = (to_f(x[a]) - c.m) * R.inv_t - c.logz, p = expf(lp);
-            float extra = 0.f;
-            bool on = false;
-            for (int k = 0; k < listed; ++k)
-                if (idx[k] == a) {
-                    extra += add[k];
-                    on = true;
-                }
-            const float base = (on ? c.l0 : c.c0) + (p == 0.f ? 0.f : c.c1 * lp);
-            v = (p * base + extra) * R.inv_t;
-        }
-        g[a] = from_f<T>(v);
+template <bool ENT>
+__device__ __forceinline__ float grad_of(float x, const RowGrad& g, float c0, float add, float inv_t) {
+    const float lp = (x - g.m) * inv_t - g.logz, p = exp2_(lp * LOG2E);
+    // p is 0 below -104: the bound keeps 0 * inf out and changes nothing else
+    return (p * (ENT ? c0 + g.c1 * fmaxf(lp, -1e4f) : c0) + add) * inv_t;
+}
+
+// The elements of chunk c that are set in `field`, the others 0.
+template <typename T, bool ENT>
+__device__ __forceinline__ void grad_chunk(const T* x, T* g, int first, int a, uint32_t field, const RowGrad& r,
+                                           float inv_t) {
+    constexpr int E = Chunk<T>::E;
+    const bool full = first >= 0 && first + E <= a;
+    Chunk<T> q;
+    if (full && ((intptr_t)(x + first) & 31) == 0) {
+        q.load(x + first);
+    } else {
+        q.fill(0);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if ((field >> e) & 1) q.set(e, to_f(x[first + e]));
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) q.set(e, (field >> e) & 1 ? grad_of<ENT>(q.get(e), r, r.c0, 0.f, inv_t) : 0.f);
+    if (full) {
+        q.store(g + first);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (first + e >= 0 && first + e < a) g[first + e] = from_f<T>(q.get(e));
     }
 }
 
-template <typename T, int MASK>
-__global__ void __launch_bounds__(PT) logprobs_backward_kernel(Rows R, sb_logprobs f, sb_logprobs_grad g) {
-    __shared__ int idx[SB_POLICY_MAX_TOP + 1];
-    __shared__ float add[SB_POLICY_MAX_TOP + 1];
-    for (int64_t row = blockIdx.x; row < R.n; row += gridDim.x) {
-        const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        const uint8_t* m = R.mask + row * R.mask_stride;
-        __syncthreads();
-        if (threadIdx.x <= f.top) {
-            int64_t a = -1;
-            float v = 0.f;
-            if (threadIdx.x < f.top) {
-                if (g.g_top) {
-                    a = f.top_action[row * f.top + threadIdx.x];
-                    v = g.g_top[row * f.top + threadIdx.x];
-                }
-            } else if (g.g_logprob) {
-                a = load_index(f.actions, f.action_bytes, row);
-                if (a < 0 || a >= R.a || !legal<MASK>(m, (int)a)) a = -1;
-                v = g.g_logprob[row * g.g_logprob_stride];
-            }
-            idx[threadIdx.x] = (int)a;
-            add[threadIdx.x] = a < 0 ? 0.f : v;
+// A warp's part of a gradient row: the 32-byte chunks of the row as it lies
+// in memory, so that every sector but the row's first and last is stored
+// whole and once.  Chunks without a legal action are zeros; the others are
+// listed and computed 32 at a time.  Returns the part's actions [lo, hi).
+template <typename T, int MASK, int W, bool ENT>
+__device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, const RowGrad& r, float inv_t,
+                                         uint32_t* list, int part) {
+    constexpr int E = Chunk<T>::E;
+    const int lane = threadIdx.x & 31;
+    const int e0 = (int)(((intptr_t)g & 31) / sizeof(T));
+    const int chunks = (a + e0 + E - 1) / E, per = (chunks + W - 1) / W;
+    const int lo = part * per, hi = min(chunks, lo + per);
+    if (MASK == SB_MASK_NONE) {
+        for (int ch = lo + lane; ch < hi; ch += 32) {
+            const int first = ch * E - e0;
+            const uint32_t head = first < 0 ? ALL << -first : ALL;
+            const uint32_t tail = first + E > a ? ALL >> (32 - (a - first)) : ALL;
+            grad_chunk<T, ENT>(x, g, first, a, head & tail & ((1u << E) - 1u), r, inv_t);
         }
-        __syncthreads();
-        float total = 0.f;
-        for (int k = 0; k <= f.top; ++k) total += add[k];
+    } else {
+        Chunk<T> zero;
+        zero.fill(0);
+        int count = 0;
+        for (int c0 = lo; c0 < hi; c0 += 32) {
+            const int ch = c0 + lane, first = ch * E - e0;
+            const uint32_t f = ch < hi ? bits.field(first, E) : 0u;
+            const bool full = first >= 0 && first + E <= a;
+            const bool put = ch < hi && (f != 0 || !full);
+            const unsigned b = __ballot_sync(ALL, put);
+            if (put) list[count + __popc(b & ((1u << lane) - 1u))] = (uint32_t)ch | f << 16;
+            else if (ch < hi) zero.store(g + first);
+            count += __popc(b);
+            if (count > CHUNKS - 32 || c0 + 32 >= hi) {
+                __syncwarp();
+                for (int i = lane; i < count; i += 32) {
+                    const uint32_t v = list[i];
+                    grad_chunk<T, ENT>(x, g, (int)(v & 0xffffu) * E - e0, a, v >> 16, r, inv_t);
+                }
+                __syncwarp();
+                count = 0;
+            }
+        }
+    }
+    __syncwarp();  // the listed actions' own values are stored over these
+    return make_int2(max(0, lo * E - e0), hi * E - e0);
+}
+
+template <typename T, int MASK, int W>
+__global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, sb_logprobs f, sb_logprobs_grad g) {
+    extern __shared__ uint4 dyn[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
+    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
+    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
+    uint32_t* list = reinterpret_cast<uint32_t*>(sh + (WARPS / W) * row_bytes) + warp * CHUNKS;
+    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
+    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
+        const T* x = static_cast<const T*>(R.x) + row * R.stride;
+        T* out = static_cast<T*>(g.grad) + row * R.a;
+        // lane k < top holds alternative k; the given action's share joins the
+        // alternative that is the same action, or stays alone
+        int mine = -1;
+        float add = 0.f;
+        if (g.g_top && lane < f.top) {
+            mine = (int)f.top_action[row * f.top + lane];
+            if (mine >= 0) add = g.g_top[row * f.top + lane];
+        }
+        int64_t act = -1;
+        float ga = 0.f;
+        if (g.g_logprob) {
+            act = load_index(f.actions, f.action_bytes, row);
+            ga = g.g_logprob[row * g.g_logprob_stride];
+        }
         const float gh = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] : 0.f;
-        RowGrad c = {f.row_stats[2 * row], f.row_stats[2 * row + 1], -(total + gh * f.entropy[row]), -gh, 0.f};
-        c.l0 = c.c0;
-        write_grad<T, MASK>(R, x, m, static_cast<T*>(g.grad) + row * R.a, c, f.top + 1, idx, add);
+        const float2 st = *reinterpret_cast<const float2*>(f.row_stats + 2 * row);
+        const float h = f.entropy[row];
+        Bits bits = {nullptr, 0};
+        if (MASK != SB_MASK_NONE) {
+            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            if (W == 1) __syncwarp();
+            else __syncthreads();
+        }
+        bool legal = act >= 0 && act < R.a;
+        if (MASK != SB_MASK_NONE) legal = legal && bits.test((int)act);
+        const float total = warp_sum(add) + (legal ? ga : 0.f);
+        const RowGrad r = {st.x, st.y, -(total + gh * h), -gh, -(total + gh * h)};
+        const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, list, W == 1 ? 0 : warp);
+        const bool same = legal && mine == (int)act;
+        if (same) add += ga;
+        if (mine >= own.x && mine < own.y) out[mine] = from_f<T>(grad_of<true>(to_f(x[mine]), r, r.l0, add, R.inv_t));
+        if (!__any_sync(ALL, same) && lane == 0 && legal && act >= own.x && act < own.y)
+            out[act] = from_f<T>(grad_of<true>(to_f(x[act]), r, r.l0, ga, R.inv_t));
+        if (W > 1) __syncthreads();
+        else __syncwarp();
     }
 }
 
-// The kept teacher entries of a row in shared memory: idx < 0 where one is
-// left out, q its weight; returns the sum of the weights.
+// ---- distillation ------------------------------------------------------------------------
+
+// Kept per row for the backward pass: (M, log Z), (Q, Q - q_r / p_r) and the
+// teacher's own (maximum, log sum).
+
+// Teacher entry k of a row: its action (-1 where it is left out) and logit.
 template <int MASK>
-__device__ float load_teacher(const Rows& R, const uint8_t* m, const sb_distill& d, int64_t row, int* idx, float* q,
-                              Sum* sh, float* tm, float* tz) {
-    __syncthreads();
-    Sum s = empty_sum();
-    for (int k = threadIdx.x; k < d.listed; k += PT) {
-        const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
-        const float v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
-        const bool keep = a >= 0 && a < R.a && legal<MASK>(m, (int)a) && !(v == NEG_INF);
-        idx[k] = keep ? (int)a : -1;
-        q[k] = v;
-        if (keep) s = merge(s, one(v), R.inv_t);
-    }
-    *tm = 0.f;
-    *tz = 0.f;
-    if (!d.tail) {
-        s = block_merge(s, R.inv_t, sh);
-        const float2 st = stats_of(s);
-        *tm = st.x;
-        *tz = st.y;
-    }
-    __syncthreads();
-    float total = 0.f;
-    for (int k = 0; k < d.listed; ++k)
-        if (idx[k] >= 0) total += expf((q[k] - *tm) * (d.tail ? 1.f : R.inv_t) - *tz);
-    return total;
+__device__ __forceinline__ int teacher(const Rows& R, const sb_distill& d, Bits bits, int64_t row, int k, float* v) {
+    if (k >= d.listed) return -1;
+    const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
+    *v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
+    if (a < 0 || a >= R.a || *v == NEG_INF) return -1;
+    if (MASK != SB_MASK_NONE && !bits.test((int)a)) return -1;
+    return (int)a;
 }
 
-template <typename T, int MASK>
-__global__ void __launch_bounds__(PT) distill_kernel(Rows R, sb_distill d) {
-    __shared__ Sum sh[PT / 32];
-    __shared__ int idx[SB_POLICY_MAX_TEACHER];
-    __shared__ float val[SB_POLICY_MAX_TEACHER];
-    for (int64_t row = blockIdx.x; row < R.n; row += gridDim.x) {
+template <typename T, int MASK, int W, bool TAIL>
+__global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill d) {
+    extern __shared__ uint4 dyn[];
+    __shared__ Sum sums[WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = W == 1 ? lane : threadIdx.x;
+    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
+    const int row_bytes = bits_bytes(R.a) * ((MASK != SB_MASK_NONE) + TAIL);
+    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
+    uint32_t* sh_skip = reinterpret_cast<uint32_t*>(sh_bits + (MASK != SB_MASK_NONE ? bits_bytes(R.a) : 0));
+    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
+    const float c = R.inv_t * LOG2E, tc = TAIL ? 1.f : R.inv_t;
+    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
+    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        const uint8_t* m = R.mask + row * R.mask_stride;
-        float tm, tz;
-        const float sq = load_teacher<MASK>(R, m, d, row, idx, val, sh, &tm, &tz);
-        Sum rest = empty_sum(), in = empty_sum();
-        for (int a = threadIdx.x; a < R.a; a += PT) {
-            if (!legal<MASK>(m, a)) continue;
-            bool on = false;
-            for (int k = 0; k < d.listed; ++k) on |= idx[k] == a;
-            if (on) in = merge(in, one(to_f(x[a])), R.inv_t);
-            else rest = merge(rest, one(to_f(x[a])), R.inv_t);
-        }
-        in = block_merge(in, R.inv_t, sh);
-        rest = block_merge(rest, R.inv_t, sh);
-        const float2 st = stats_of(merge(in, rest, R.inv_t));
-        float total = sq, loss = 0.f, share = 0.f;
-        if (d.tail) {
-            const bool left = rest.m > NEG_INF || rest.r != rest.r;
-            const float qr = left ? fmaxf(0.f, 1.f - sq) : 0.f;
-            if (qr > 0.f) {
-                const float2 si = stats_of(in), sr = stats_of(rest);
-                const float sp = expf((si.x - st.x) * R.inv_t + si.y - st.y);
-                const float lpr = in.m == NEG_INF ? 0.f
-                                  : sp < 0.5f     ? log1pf(-sp)
-                                                  : (sr.x - st.x) * R.inv_t + sr.y - st.y;
-                const float lqr = log1pf(-sq);
-                loss = qr * (lqr - lpr);
-                share = expf(lqr - lpr);
-                total += qr;
-            }
-        }
-        if (threadIdx.x == 0) {
-            for (int k = 0; k < d.listed; ++k)
-                if (idx[k] >= 0) {
-                    const float lq = (val[k] - tm) * (d.tail ? 1.f : R.inv_t) - tz;
-                    loss += expf(lq) * (lq - ((to_f(x[idx[k]]) - st.x) * R.inv_t - st.y));
+        Bits bits = {nullptr, 0};
+        if (MASK != SB_MASK_NONE) bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, tid);
+        if (TAIL)
+            for (int i = tid; i < bits_bytes(R.a) / 4; i += 32 * W) sh_skip[i] = 0;
+        if (W == 1) __syncwarp();
+        else __syncthreads();
+        const Bits skip = {sh_skip, bits.p};
+        // the teacher's weights, and which entry is an action's first
+        Sum ts = no_sum();
+        float sq = 0.f;
+        unsigned first = 0;  // bit j: this lane's entry of round j
+        if (W == 1 || warp == 0) {
+            for (int k0 = 0, j = 0; k0 < d.listed; k0 += 32, ++j) {
+                float v = 0.f;
+                const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
+                if (TAIL) {
+                    if (a >= 0) sq += expf(v);
+                    const unsigned peers = __match_any_sync(ALL, a);
+                    const bool lead = a >= 0 && (peers & ((1u << lane) - 1u)) == 0 && !skip.test(a);
+                    __syncwarp();
+                    if (lead) {
+                        first |= 1u << j;
+                        atomicOr(&sh_skip[(a + skip.p) >> 5], 1u << ((a + skip.p) & 31));
+                    }
+                    __syncwarp();
+                } else {
+                    float t[1] = {a >= 0 ? v : NEG_INF};
+                    take<1, false>(ts, t, c);
                 }
-            d.loss[row] = loss;
-            if (d.row_stats) {
-                float* s = d.row_stats + 6 * row;
-                s[0] = st.x;
-                s[1] = st.y;
-                s[2] = total;
-                s[3] = total - share;
-                s[4] = tm;
-                s[5] = tz;
             }
         }
+        if (TAIL && W > 1) __syncthreads();
+        Sum s = no_sum();
+        Top none;
+        if (MASK == SB_MASK_NONE) pass_all<T, W, false, false>(s, none, x, TAIL ? &skip : nullptr, R.a, c, W == 1 ? 0 : warp);
+        else pass_masked<T, W, false, false>(s, none, x, bits, TAIL ? sh_skip : nullptr, R.a, c, list, W == 1 ? 0 : warp);
+        s = whole<W>(s, c, sums);
+        if (W == 1 || warp == 0) {
+            Sum all = s, in = no_sum();
+            float2 tst = make_float2(0.f, 0.f);
+            if (TAIL) {
+                sq = warp_sum(sq);
+                for (int k0 = 0, j = 0; k0 < d.listed; k0 += 32, ++j) {
+                    float v = 0.f;
+                    const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
+                    float t[1] = {(first >> j) & 1 ? to_f(x[a]) : NEG_INF};
+                    take<1, false>(in, t, c);
+                }
+                in = whole<1>(in, c, nullptr);
+                all = join(in, s, c);
+            } else {
+                tst = stats_of(whole<1>(ts, c, nullptr));
+            }
+            const float2 st = stats_of(all);
+            float loss = 0.f, kept = 0.f;
+            for (int k0 = 0; k0 < d.listed; k0 += 32) {
+                float v = 0.f;
+                const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
+                if (a >= 0) {
+                    const float lq = (v - tst.x) * tc - tst.y, q = expf(lq);
+                    loss += q * (lq - ((to_f(x[a]) - st.x) * R.inv_t - st.y));
+                    kept += q;
+                }
+            }
+            loss = warp_sum(loss);
+            float total = TAIL ? sq : warp_sum(kept), share = 0.f;
+            if (TAIL) {
+                // the unlisted actions as one: q_r log(q_r / p_r), each log from
+                // the side that keeps its digits
+                const float qr = s.m > NEG_INF || s.r != s.r ? fmaxf(0.f, 1.f - sq) : 0.f;
+                if (qr > 0.f) {
+                    const float2 si = stats_of(in), sr = stats_of(s);
+                    const float sp = expf((si.x - st.x) * R.inv_t + si.y - st.y);
+                    const float lpr = in.m == NEG_INF ? 0.f
+                                      : sp < 0.5f     ? log1pf(-sp)
+                                                      : (sr.x - st.x) * R.inv_t + sr.y - st.y;
+                    const float lqr = log1pf(-sq);
+                    loss += qr * (lqr - lpr);
+                    share = expf(lqr - lpr);
+                    total += qr;
+                }
+            }
+            if (lane == 0) {
+                d.loss[row] = loss;
+                if (d.row_stats) {
+                    float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
+                    o[0] = st;
+                    o[1] = make_float2(total, total - share);
+                    o[2] = tst;
+                }
+            }
+        }
+        if (W > 1) __syncthreads();
+        else __syncwarp();
     }
 }
 
-template <typename T, int MASK>
-__global__ void __launch_bounds__(PT) distill_backward_kernel(Rows R, sb_distill d, const float* g_loss,
-                                                              int64_t g_stride, T* grad) {
-    __shared__ int idx[SB_POLICY_MAX_TEACHER];
-    __shared__ float add[SB_POLICY_MAX_TEACHER];
-    for (int64_t row = blockIdx.x; row < R.n; row += gridDim.x) {
+template <typename T, int MASK, int W>
+__global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb_distill d, const float* g_loss,
+                                                                      int64_t g_stride, T* grad) {
+    extern __shared__ uint4 dyn[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
+    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
+    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
+    uint32_t* list = reinterpret_cast<uint32_t*>(sh + (WARPS / W) * row_bytes) + warp * CHUNKS;
+    const float tc = d.tail ? 1.f : R.inv_t;
+    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
+    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        const uint8_t* m = R.mask + row * R.mask_stride;
-        const float* s = d.row_stats + 6 * row;
+        T* out = grad + row * R.a;
+        const float2* s = reinterpret_cast<const float2*>(d.row_stats + 6 * row);
+        const float2 st = s[0], co = s[1], te = s[2];
         const float w = g_loss[row * g_stride];
-        __syncthreads();
-        for (int k = threadIdx.x; k < d.listed; k += PT) {
-            const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
-            const float v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
-            const bool keep = a >= 0 && a < R.a && legal<MASK>(m, (int)a) && !(v == NEG_INF);
-            idx[k] = keep ? (int)a : -1;
-            add[k] = -w * expf((v - s[4]) * (d.tail ? 1.f : R.inv_t) - s[5]);
+        Bits bits = {nullptr, 0};
+        if (MASK != SB_MASK_NONE) {
+            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            if (W == 1) __syncwarp();
+            else __syncthreads();
         }
-        __syncthreads();
-        RowGrad c = {s[0], s[1], w * s[3], 0.f, w * s[2]};
-        write_grad<T, MASK>(R, x, m, grad + row * R.a, c, d.listed, idx, add);
+        const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
+        const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, list, W == 1 ? 0 : warp);
+        for (int k0 = 0; k0 < d.listed; k0 += 32) {
+            float v = 0.f;
+            const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
+            float q = 0.f;
+            // an action that is listed again takes all of its entries' weights:
+            // every one of them stores the same value, summed in the same order
+            for (int j0 = 0; j0 < d.listed; j0 += 32) {
+                float u = 0.f;
+                const int b = j0 == k0 ? a : teacher<MASK>(R, d, bits, row, j0 + lane, &u);
+                if (j0 == k0) u = v;
+                const float qu = b >= 0 ? expf((u - te.x) * tc - te.y) : 0.f;
+                for (int j = 0; j < 32 && j0 + j < d.listed; ++j) {
+                    const int bj = __shfl_sync(ALL, b, j);
+                    const float qj = __shfl_sync(ALL, qu, j);
+                    if (a >= 0 && bj == a) q += qj;
+                }
+            }
+            if (a >= 0 && a >= own.x && a < own.y)
+                out[a] = from_f<T>(grad_of<false>(to_f(x[a]), r, r.l0, -w * q, R.inv_t));
+        }
+        if (W > 1) __syncthreads();
+        else __syncwarp();
     }
 }
 
@@ -379,21 +837,37 @@ int launched(const char* what) {
     return e == cudaSuccess ? SB_OK : cuda_fail(e, what);
 }
 
-unsigned grid_of(int64_t rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
+unsigned grid_of(int64_t rows, int w) {
+    const int64_t ctas = (rows + WARPS / w - 1) / (WARPS / w);
+    return (unsigned)(ctas < 0x7fffffff ? ctas : 0x7fffffff);
+}
 
-// Call f with the logits' element type and the mask kind as constants.
+template <int V> using Const = std::integral_constant<int, V>;
+
+// Call f(element type, mask kind, warps per row) as constants: four warps
+// where one would have more than ROW_BYTES to stream for a row.
 template <typename F>
-int dispatch(const sb_logits* x, F f) {
-#define SB_KINDS(T)                                                                                     \
-    switch (x->mask_kind) {                                                                             \
-        case SB_MASK_U8: return f((T*)nullptr, std::integral_constant<int, SB_MASK_U8>{});              \
-        case SB_MASK_BITS: return f((T*)nullptr, std::integral_constant<int, SB_MASK_BITS>{});          \
-        default: return f((T*)nullptr, std::integral_constant<int, SB_MASK_NONE>{});                    \
-    }
-    if (x->dtype == SB_DTYPE_F32) SB_KINDS(float)
-    if (x->dtype == SB_DTYPE_BF16) SB_KINDS(__nv_bfloat16)
-    SB_KINDS(__half)
-#undef SB_KINDS
+int dispatch(const sb_logits* x, int64_t bytes, F f) {
+    const bool wide = bytes > ROW_BYTES;
+    auto kinds = [&](auto* t) {
+        switch (x->mask_kind) {
+            case SB_MASK_U8: return wide ? f(t, Const<SB_MASK_U8>{}, Const<WARPS>{}) : f(t, Const<SB_MASK_U8>{}, Const<1>{});
+            case SB_MASK_BITS:
+                return wide ? f(t, Const<SB_MASK_BITS>{}, Const<WARPS>{}) : f(t, Const<SB_MASK_BITS>{}, Const<1>{});
+            default: return wide ? f(t, Const<SB_MASK_NONE>{}, Const<WARPS>{}) : f(t, Const<SB_MASK_NONE>{}, Const<1>{});
+        }
+    };
+    if (x->dtype == SB_DTYPE_F32) return kinds((float*)nullptr);
+    if (x->dtype == SB_DTYPE_BF16) return kinds((__nv_bfloat16*)nullptr);
+    return kinds((__half*)nullptr);
+}
+
+int64_t row_bytes(const sb_logits* x) { return (int64_t)x->n_actions * (x->dtype == SB_DTYPE_F32 ? 4 : 2); }
+
+// What a forward pass streams of a row whatever it holds.
+int64_t read_bytes(const sb_logits* x) {
+    if (x->mask_kind == SB_MASK_U8) return x->n_actions;
+    return x->mask_kind == SB_MASK_BITS ? (x->n_actions + 7) / 8 : row_bytes(x);
 }
 
 int check_logprobs(const sb_logits* x, const sb_logprobs* o) {
@@ -417,6 +891,7 @@ int check_distill(const sb_logits* x, const sb_distill* d) {
     if (!aligned(d->teacher_actions, d->action_bytes) ||
         !aligned(d->teacher_logits, d->teacher_dtype == SB_DTYPE_F32 ? 4 : 2))
         return fail(SB_E_ARG, "teacher actions or logits not aligned to their type");
+    if (d->row_stats && !aligned(d->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
     return SB_OK;
 }
 
@@ -434,9 +909,15 @@ int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream)
     if (!out->entropy || (out->actions != nullptr) != (out->logprob != nullptr))
         return fail(SB_E_ARG, "entropy is NULL, or actions and logprob disagree");
     if (out->top && (!out->top_action || !out->top_logprob)) return fail(SB_E_ARG, "top outputs are NULL");
-    return dispatch(x, [&](auto* t, auto mask) {
+    if (out->row_stats && !aligned(out->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
+    return dispatch(x, read_bytes(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
-        logprobs_kernel<T, decltype(mask)::value><<<grid_of(R.n), PT, 0, (cudaStream_t)stream>>>(R, *out);
+        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 2 * LIST;
+        if (out->top)
+            logprobs_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
+        else
+            logprobs_kernel<T, M, W, false><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
         return launched("logprobs_kernel launch");
     });
 }
@@ -449,11 +930,14 @@ int sb_action_logprobs_backward(const sb_logits* x, const sb_logprobs* fwd, cons
     if (x->n_rows == 0) return SB_OK;
     if (!g->grad || !fwd->row_stats || !fwd->entropy) return fail(SB_E_ARG, "grad, row_stats or entropy is NULL");
     if (!aligned(g->grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
+    if (!aligned(fwd->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
     if ((g->g_logprob && !fwd->actions) || (g->g_top && (!fwd->top || !fwd->top_action)))
         return fail(SB_E_ARG, "a gradient of an output that the forward call did not have");
-    return dispatch(x, [&](auto* t, auto mask) {
+    return dispatch(x, row_bytes(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
-        logprobs_backward_kernel<T, decltype(mask)::value><<<grid_of(R.n), PT, 0, (cudaStream_t)stream>>>(R, *fwd, *g);
+        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 4 * CHUNKS;
+        logprobs_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *fwd, *g);
         return launched("logprobs_backward_kernel launch");
     });
 }
@@ -463,9 +947,15 @@ int sb_distill_loss(const sb_logits* x, const sb_distill* d, void* stream) {
     int rc = check_rows(x, &R);
     if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
     if (!d->loss) return fail(SB_E_ARG, "loss is NULL");
-    return dispatch(x, [&](auto* t, auto mask) {
+    return dispatch(x, read_bytes(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
-        distill_kernel<T, decltype(mask)::value><<<grid_of(R.n), PT, 0, (cudaStream_t)stream>>>(R, *d);
+        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
+        const int lists = M == SB_MASK_NONE ? 0 : WARPS * 2 * LIST;
+        const int smem = WARPS / W * bits_bytes(R.a) * ((M != SB_MASK_NONE) + d->tail) + lists;
+        if (d->tail)
+            distill_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *d);
+        else
+            distill_kernel<T, M, W, false><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *d);
         return launched("distill_kernel launch");
     });
 }
@@ -477,9 +967,11 @@ int sb_distill_loss_backward(const sb_logits* x, const sb_distill* d, const floa
     if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
     if (!g_loss || !grad || !d->row_stats) return fail(SB_E_ARG, "g_loss, grad or row_stats is NULL");
     if (!aligned(grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
-    return dispatch(x, [&](auto* t, auto mask) {
+    return dispatch(x, row_bytes(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
-        distill_backward_kernel<T, decltype(mask)::value><<<grid_of(R.n), PT, 0, (cudaStream_t)stream>>>(
+        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 4 * CHUNKS;
+        distill_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(
             R, *d, g_loss, g_loss_stride, static_cast<T*>(grad));
         return launched("distill_backward_kernel launch");
     });

@@ -13,9 +13,9 @@
 // first, so large logits lose nothing).
 //
 // Layout of the work: a row belongs to one warp, or to the four warps of a
-// CTA where the bytes that a lane has to stream would make a long chain (more
-// than ROW_BYTES per row).  That rule looks at the shape and the types alone,
-// so a row's bits do not depend on the batch it comes in.  A legal mask is
+// CTA where it is long (wide_forward, wide_backward).  That rule looks at the
+// shape and the types alone, so a row's bits do not depend on the batch it
+// comes in.  A legal mask is
 // staged in shared memory as one bit per action, and only the logits of set
 // bits are read: a position has some 30 legal moves of 10,000, so a row costs
 // its mask and 30 sectors instead of 20 or 40 KB.
@@ -34,13 +34,13 @@ namespace sb {
 namespace {
 
 constexpr int WARPS = 4;                  // warps of a CTA: one row each, or one row together
-constexpr int ROW_BYTES = 4096;
 constexpr unsigned ALL = 0xffffffffu;
 constexpr float NEG_INF = -INFINITY;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int LIST = 1024;                // legal actions a warp gathers at once
-constexpr int BLOCK_WORDS = 8;            // mask words of a lane between two gathers
-constexpr int CHUNKS = 128;               // gradient chunks a warp lists at once
+constexpr int BLOCK_WORDS = 11;           // mask words of a lane between two gathers (odd: no bank conflicts)
+constexpr int CHUNKS = 64;                // gradient chunks a warp lists at once
+constexpr int SLOT = 48;                  // bytes between two lanes' chunk slots (32 used)
 
 struct Rows {
     const void* x;
@@ -131,6 +131,11 @@ struct Bits {
     uint32_t* w;
     int p;
     __device__ __forceinline__ bool test(int a) const { return (w[(a + p) >> 5] >> ((a + p) & 31)) & 1; }
+    // the 32 actions from 32 i on
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const int b = 32 * i + p;
+        return __funnelshift_r(w[b >> 5], w[(b >> 5) + 1], b & 31);
+    }
     // `len` <= 16 bits of the actions from a on (a >= -16)
     __device__ __forceinline__ uint32_t field(int a, int len) const {
         const int b = a + p;
@@ -281,10 +286,15 @@ struct Top {
         a = bar_a = 0x7fffffff;
         k = n;
     }
+    __device__ __forceinline__ void set_bar() {
+        bar_x = __shfl_sync(ALL, x, k - 1);
+        bar_a = __shfl_sync(ALL, a, k - 1);
+    }
     __device__ __forceinline__ bool wants(float v, int b) const {
         return v > bar_x || (v == bar_x && b < bar_a && v > NEG_INF);
     }
-    __device__ __noinline__ void offer(float v, int b) {  // one candidate per lane (-inf: none)
+    // One candidate per lane (-inf: none), put in place one by one.
+    __device__ __forceinline__ void offer(float v, int b) {
         unsigned c = __ballot_sync(ALL, wants(v, b));
         while (c) {
             const int src = __ffs(c) - 1;
@@ -298,32 +308,58 @@ struct Top {
                 x = lane == at ? cx : ux;
                 a = lane == at ? ca : ua;
             }
-            bar_x = __shfl_sync(ALL, x, k - 1);
-            bar_a = __shfl_sync(ALL, a, k - 1);
+            set_bar();
             c &= c - 1;
             c &= __ballot_sync(ALL, wants(v, b));
         }
+    }
+    // The first 32 candidates of an empty list: a bitonic sort (15 exchanges
+    // instead of up to 32 insertions).
+    __device__ __forceinline__ void fill(float v, int b) {
+        const int lane = threadIdx.x & 31;
+        x = v == v ? v : NEG_INF;
+        a = x > NEG_INF ? b : 0x7fffffff;
+#pragma unroll
+        for (int n = 2; n <= 32; n <<= 1) {
+#pragma unroll
+            for (int d = n >> 1; d; d >>= 1) {
+                const float ox = __shfl_xor_sync(ALL, x, d);
+                const int oa = __shfl_xor_sync(ALL, a, d);
+                const bool mine_first = x > ox || (x == ox && a < oa);
+                const bool keep_first = ((lane & d) == 0) == ((lane & n) == 0);
+                if (mine_first != keep_first) {
+                    x = ox;
+                    a = oa;
+                }
+            }
+        }
+        set_bar();
     }
 };
 
 // ---- one pass over a row ------------------------------------------------------------
 
-// The legal logits of this warp's part of a row: `w` of W parts.  `skip`
-// holds bits (laid out like the mask's) of actions to leave out, or NULL.
-template <typename T, int W, bool ENT, bool TOP>
-__device__ __forceinline__ void pass_masked(Sum& s, Top& top, const T* x, Bits bits, const uint32_t* skip, int a, float c,
-                                            uint16_t* list, int part) {
+// The legal logits of this warp's blocks of a row (block b is warp b % W's).
+// The legal actions are listed in ascending order and dealt to the lanes in
+// turn, so the sums' order, and with it every bit of the result, is the same
+// for any kind of mask and wherever its rows lie.  SKIP leaves out the
+// actions of `skip`.  Returns how many actions were taken.
+template <typename T, int W, bool ENT, bool TOP, bool SKIP>
+__device__ __forceinline__ int pass_masked(Sum& s, Top& top, const T* x, Bits bits, Bits skip, int a, float c,
+                                           uint16_t* list, int part) {
     const int lane = threadIdx.x & 31;
-    const int words = (bits.p + a + 31) >> 5;
-    for (int w0 = part * 32; w0 < words; w0 += 32 * BLOCK_WORDS * W) {
-        // lane's words: w0 + lane + k * 32 * W
-        uint32_t w[BLOCK_WORDS];
+    const int words = (a + 31) >> 5;
+    auto word = [&](int i) { return i >= words ? 0u : SKIP ? bits.word(i) & ~skip.word(i) : bits.word(i); };
+    int taken = 0;
+    for (int w0 = part * 32 * BLOCK_WORDS; w0 < words; w0 += 32 * BLOCK_WORDS * W) {
+        const int mine = w0 + lane * BLOCK_WORDS;
+        uint32_t some = 0;  // bit k: the lane's word k is not 0
         int count = 0;
 #pragma unroll
         for (int k = 0; k < BLOCK_WORDS; ++k) {
-            const int i = w0 + lane + k * 32 * W;
-            w[k] = i < words ? bits.w[i] & (skip ? ~skip[i] : ALL) : 0u;
-            count += __popc(w[k]);
+            const uint32_t w = word(mine + k);
+            count += __popc(w);
+            some |= w ? 1u << k : 0u;
         }
         int at = count;
 #pragma unroll
@@ -332,106 +368,160 @@ __device__ __forceinline__ void pass_masked(Sum& s, Top& top, const T* x, Bits b
             if (lane >= o) at += v;
         }
         const int total = __shfl_sync(ALL, at, 31);
+        if (total == 0) continue;
+        const bool first = taken == 0;
+        taken += total;
         if (total <= LIST) {
             at -= count;
-#pragma unroll
-            for (int k = 0; k < BLOCK_WORDS; ++k) {
-                const int base = (w0 + lane + k * 32 * W) * 32 - bits.p;
-                while (w[k]) {
-                    list[at++] = (uint16_t)(base + __ffs(w[k]) - 1);
-                    w[k] &= w[k] - 1;
+            uint32_t w = 0;
+            int base = 0;
+            while (some | w) {  // one action a turn, whichever word it is in
+                if (!w) {
+                    const int i = mine + __ffs(some) - 1;
+                    some &= some - 1;
+                    w = word(i);
+                    base = i * 32;
                 }
+                list[at++] = (uint16_t)(base + __ffs(w) - 1);
+                w &= w - 1;
             }
             __syncwarp();
-            for (int i = 0; i < total; i += 128) {
-                float v[4];
-                int b[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int n = i + q * 32 + lane;
-                    b[q] = n < total ? list[n] : 0;
-                    v[q] = n < total ? to_f(x[b[q]]) : NEG_INF;
+            if (TOP || total <= 32) {
+                for (int i = 0; i < total; i += 32) {
+                    const int b = i + lane < total ? list[i + lane] : 0;
+                    const float v[1] = {i + lane < total ? to_f(x[b]) : NEG_INF};
+                    take<1, ENT>(s, v, c);
+                    if (TOP) {
+                        if (first && i == 0) top.fill(v[0], b);
+                        else top.offer(v[0], b);
+                    }
                 }
-                take<4, ENT>(s, v, c);
-                if (TOP)
+            } else {
+                for (int i = 0; i < total; i += 128) {
+                    float v[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) top.offer(v[q], b[q]);
+                    for (int q = 0; q < 4; ++q) {
+                        const int n = i + q * 32 + lane;
+                        v[q] = n < total ? to_f(x[list[n]]) : NEG_INF;
+                    }
+                    take<4, ENT>(s, v, c);
+                }
             }
             __syncwarp();
         } else {
             // too many for the list: every word's 32 actions in turn, a lane each
+            const int end = min(words, w0 + 32 * BLOCK_WORDS);
+            float best = NEG_INF;
+            for (int i = w0; i < end; i += 8) {
+                float v[8];
 #pragma unroll
-            for (int k = 0; k < BLOCK_WORDS; ++k) {
-                const int base = (w0 + k * 32 * W) * 32 - bits.p + lane;
-                if (!__any_sync(ALL, w[k])) continue;
-                for (int j = 0; j < 32; j += 8) {
-                    float v[8];
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const uint32_t m = __shfl_sync(ALL, w[k], j + q);
-                        v[q] = (m >> lane) & 1 ? to_f(x[base + 32 * (j + q)]) : NEG_INF;
+                for (int q = 0; q < 8; ++q) {
+                    const uint32_t m = i + q < end ? word(i + q) : 0u;
+                    v[q] = (m >> lane) & 1 ? to_f(x[(i + q) * 32 + lane]) : NEG_INF;
+                    best = fmaxf(best, v[q]);
+                }
+                take<8, ENT>(s, v, c);
+            }
+            if (TOP) {
+                // only a lane whose best reaches the k-th best of what the list
+                // holds and of all lanes' bests can hold one of the k best
+                Top bar = top;
+                bar.offer(best, lane);
+                unsigned who = __ballot_sync(ALL, best >= bar.bar_x && best > NEG_INF);
+                for (; who; who &= who - 1) {
+                    const int src = __ffs(who) - 1;
+                    for (int i = w0; i < end; i += 32) {
+                        const int b = (i + lane) * 32 + src;
+                        const uint32_t m = i + lane < end ? word(i + lane) : 0u;
+                        top.offer((m >> src) & 1 ? to_f(x[b]) : NEG_INF, b);
                     }
-                    take<8, ENT>(s, v, c);
-                    if (TOP)
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) top.offer(v[q], base + 32 * (j + q));
                 }
             }
         }
     }
+    return taken;
 }
 
 // The same without a mask: 32-byte chunks of the row at their alignment in
-// memory, the ends that do not fill one by single loads.
-template <typename T, int W, bool ENT, bool TOP>
-__device__ __forceinline__ void pass_all(Sum& s, Top& top, const T* x, const Bits* skip, int a, float c, int part) {
+// memory, the ends that do not fill one by single loads.  Returns the lane's
+// largest logit.
+template <typename T> struct Span {
+    int head, chunks;
+    __device__ __forceinline__ Span(const T* x, int a) {
+        head = min(a, (int)((-(intptr_t)x & 31) / sizeof(T)));
+        chunks = (a - head) / Chunk<T>::E;
+    }
+};
+
+template <typename T, int W, bool ENT, bool SKIP>
+__device__ __forceinline__ float pass_all(Sum& s, const T* x, Bits skip, int a, float c, int part) {
     constexpr int E = Chunk<T>::E, U = 32 / E;
     const int lane = threadIdx.x & 31;
-    const int head = min(a, (int)((-(intptr_t)x & 31) / sizeof(T))), chunks = (a - head) / E;
+    const Span<T> sp(x, a);
+    float best = NEG_INF;
     if (part == 0) {  // the ends: fewer than two chunks, one element a lane
-        const int tail = head + chunks * E;
-        const int b = lane < head ? lane : tail + lane - head;
-        const bool on = b < a && !(skip && skip->test(b));
-        float v[1] = {on ? to_f(x[b]) : NEG_INF};
+        const int b = lane < sp.head ? lane : sp.chunks * E + lane;
+        const float v[1] = {b < a && !(SKIP && skip.test(b)) ? to_f(x[b]) : NEG_INF};
+        best = fmaxf(best, v[0]);
         take<1, ENT>(s, v, c);
-        if (TOP) top.offer(v[0], b);
     }
-    const T* body = x + head;
-    for (int c0 = part * 32 * U; c0 < chunks; c0 += 32 * U * W) {
-        Chunk<T> q[U];
+    const T* body = x + sp.head;
+    for (int c0 = part * 32; c0 < sp.chunks; c0 += 32 * U * W) {
         float v[32];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = c0 + u * 32 + lane;
-            if (i < chunks) q[u].load(body + i * E);
-        }
-        float m = NEG_INF;
+            const int i = c0 + u * 32 * W + lane;
+            Chunk<T> q;
+            if (i < sp.chunks) {
+                q.load(body + i * E);
+                const uint32_t out = SKIP ? skip.field(sp.head + i * E, E) : 0u;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = c0 + u * 32 + lane;
-            const uint32_t out = i >= chunks ? ALL : skip ? skip->field(head + i * E, E) : 0u;
+                for (int e = 0; e < E; ++e) v[u * E + e] = SKIP && (out >> e) & 1 ? NEG_INF : q.get(e);
+            } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                v[u * E + e] = (out >> e) & 1 ? NEG_INF : q[u].get(e);
-                m = fmaxf(m, v[u * E + e]);
+                for (int e = 0; e < E; ++e) v[u * E + e] = NEG_INF;
             }
         }
-        take<32, ENT>(s, v, c);
-        if (TOP && __any_sync(ALL, m >= top.bar_x)) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = c0 + u * 32 + lane;
-                for (int e = 0; e < E; ++e)  // read again from cache: this is the rare path
-                    top.offer(i < chunks ? to_f(body[i * E + e]) : NEG_INF, head + i * E + e);
+        for (int i = 0; i < 32; ++i) best = fmaxf(best, v[i]);
+        take<32, ENT>(s, v, c);
+    }
+    return best;
+}
+
+// The k best of an unmasked row, by one warp: `best[W * 32]` holds every
+// lane's largest logit.  The k-th largest of those bounds the k-th best of the
+// row from below, so only the lanes that reach it are looked through again
+// (about k of them, from cache).
+template <typename T, int W>
+__device__ __forceinline__ void top_of_all(Top& top, const T* x, int a, const float* best) {
+    constexpr int E = Chunk<T>::E;
+    const int lane = threadIdx.x & 31;
+    const Span<T> sp(x, a);
+    Top bar = top;
+    bar.fill(best[lane], lane);
+#pragma unroll
+    for (int w = 1; w < W; ++w) bar.offer(best[w * 32 + lane], w * 32 + lane);
+    for (int w = 0; w < W; ++w) {
+        const float mine = best[w * 32 + lane];
+        unsigned who = __ballot_sync(ALL, mine >= bar.bar_x && mine > NEG_INF);
+        for (; who; who &= who - 1) {
+            const int src = __ffs(who) - 1;
+            // its chunks are w * 32 + src + n * 32 * W, E elements of each
+            for (int i = lane; __any_sync(ALL, w * 32 + src + i / E * 32 * W < sp.chunks); i += 32) {
+                const int ch = w * 32 + src + i / E * 32 * W, b = sp.head + ch * E + i % E;
+                const float v = ch < sp.chunks ? to_f(x[b]) : NEG_INF;
+                top.offer(v >= bar.bar_x ? v : NEG_INF, b);
+            }
+            if (w == 0) {  // and its element of the row's ends
+                const int b = src < sp.head ? src : sp.chunks * E + src;
+                top.offer(lane == 0 && b < a ? to_f(x[b]) : NEG_INF, b);
             }
         }
     }
 }
 
 // ---- forward: given actions, entropy, top alternatives -----------------------------
-
-template <int MASK, int W>
-__host__ __device__ constexpr int list_bytes() { return MASK == SB_MASK_NONE ? 0 : 2 * LIST; }
 
 template <typename T, int MASK, int W, bool TOP>
 __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprobs o) {
@@ -459,15 +549,19 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
         top.init(TOP ? o.top : 1);
         bool legal = act >= 0 && act < R.a;
         if (MASK == SB_MASK_NONE) {
-            pass_all<T, W, true, TOP>(s, top, x, nullptr, R.a, c, W == 1 ? 0 : warp);
+            const float best = pass_all<T, W, true, false>(s, x, Bits{}, R.a, c, W == 1 ? 0 : warp);
+            if (TOP) {
+                top_x[warp][lane] = best;
+                if (W == 1) __syncwarp();
+            }
         } else {
             const Bits bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
             if (W == 1) __syncwarp();
             else __syncthreads();
             legal = legal && bits.test((int)act);
-            pass_masked<T, W, true, TOP>(s, top, x, bits, nullptr, R.a, c, list, W == 1 ? 0 : warp);
+            pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, W == 1 ? 0 : warp);
         }
-        if (TOP && W > 1) {
+        if (TOP && W > 1 && MASK != SB_MASK_NONE) {
             top_x[warp][lane] = top.x;
             top_a[warp][lane] = top.a;
         }
@@ -480,8 +574,9 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
                 if (o.row_stats) *reinterpret_cast<float2*>(o.row_stats + 2 * row) = st;
             }
             if (TOP) {
-                if (W > 1)
-#pragma unroll
+                if (MASK == SB_MASK_NONE)
+                    top_of_all<T, W>(top, x, R.a, top_x[W == 1 ? warp : 0]);
+                else if (W > 1)
                     for (int w = 1; w < W; ++w) top.offer(lane < o.top ? top_x[w][lane] : NEG_INF, top_a[w][lane]);
                 if (lane < o.top) {
                     const bool some = top.x > NEG_INF;
@@ -511,31 +606,63 @@ __device__ __forceinline__ float grad_of(float x, const RowGrad& g, float c0, fl
     return (p * (ENT ? c0 + g.c1 * fmaxf(lp, -1e4f) : c0) + add) * inv_t;
 }
 
-// The elements of chunk c that are set in `field`, the others 0.
+// One lane's chunk of a gradient row: the elements that are set in `field`,
+// the others 0.  Few are set: a loop over them, with the lane's slots in
+// shared memory to index by.
 template <typename T, bool ENT>
-__device__ __forceinline__ void grad_chunk(const T* x, T* g, int first, int a, uint32_t field, const RowGrad& r,
-                                           float inv_t) {
+__device__ __forceinline__ void grad_sparse(const T* x, T* g, int first, int a, uint32_t field, const RowGrad& r,
+                                            float inv_t, T* xs, T* gs) {
     constexpr int E = Chunk<T>::E;
-    const bool full = first >= 0 && first + E <= a;
+    const bool full = first >= 0 && first + E <= a, wide = full && ((intptr_t)(x + first) & 31) == 0;
+    uint4* x4 = reinterpret_cast<uint4*>(xs);
+    uint4* g4 = reinterpret_cast<uint4*>(gs);
     Chunk<T> q;
-    if (full && ((intptr_t)(x + first) & 31) == 0) {
+    if (wide) {
         q.load(x + first);
-    } else {
-        q.fill(0);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if ((field >> e) & 1) q.set(e, to_f(x[first + e]));
+        x4[0] = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
+        x4[1] = make_uint4(q.w[4], q.w[5], q.w[6], q.w[7]);
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) q.set(e, (field >> e) & 1 ? grad_of<ENT>(q.get(e), r, r.c0, 0.f, inv_t) : 0.f);
+    g4[0] = g4[1] = make_uint4(0, 0, 0, 0);
+    asm volatile("" ::: "memory");  // the slots are read by another type than they are written by
+    for (uint32_t f = field; f; f &= f - 1) {
+        const int e = __ffs(f) - 1;
+        gs[e] = from_f<T>(grad_of<ENT>(to_f(wide ? xs[e] : x[first + e]), r, r.c0, 0.f, inv_t));
+    }
+    asm volatile("" ::: "memory");
     if (full) {
+        const uint4 u = g4[0], v = g4[1];
+        q.w[0] = u.x, q.w[1] = u.y, q.w[2] = u.z, q.w[3] = u.w;
+        q.w[4] = v.x, q.w[5] = v.y, q.w[6] = v.z, q.w[7] = v.w;
         q.store(g + first);
     } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (first + e >= 0 && first + e < a) g[first + e] = from_f<T>(q.get(e));
+        for (int e = max(0, -first); e < E && first + e < a; ++e) g[first + e] = gs[e];
     }
 }
+
+// The same with every action legal.
+template <typename T, bool ENT>
+__device__ __forceinline__ void grad_dense(const T* x, T* g, int first, int a, const RowGrad& r, float inv_t) {
+    constexpr int E = Chunk<T>::E;
+    Chunk<T> q;
+    if (first >= 0 && first + E <= a) {
+        if (((intptr_t)(x + first) & 31) == 0) {
+            q.load(x + first);
+        } else {
+            q.fill(0);
+#pragma unroll
+            for (int e = 0; e < E; ++e) q.set(e, to_f(x[first + e]));
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) q.set(e, grad_of<ENT>(q.get(e), r, r.c0, 0.f, inv_t));
+        q.store(g + first);
+    } else {
+        for (int b = max(0, first); b < first + E && b < a; ++b)
+            g[b] = from_f<T>(grad_of<ENT>(to_f(x[b]), r, r.c0, 0.f, inv_t));
+    }
+}
+
+// Shared memory of a warp's gradient work: the list and two slots a lane.
+constexpr int GRAD_BYTES = 4 * CHUNKS + 2 * 32 * SLOT;
 
 // A warp's part of a gradient row: the 32-byte chunks of the row as it lies
 // in memory, so that every sector but the row's first and last is stored
@@ -543,20 +670,18 @@ __device__ __forceinline__ void grad_chunk(const T* x, T* g, int first, int a, u
 // listed and computed 32 at a time.  Returns the part's actions [lo, hi).
 template <typename T, int MASK, int W, bool ENT>
 __device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, const RowGrad& r, float inv_t,
-                                         uint32_t* list, int part) {
+                                         uint8_t* sh, int part) {
     constexpr int E = Chunk<T>::E;
     const int lane = threadIdx.x & 31;
     const int e0 = (int)(((intptr_t)g & 31) / sizeof(T));
     const int chunks = (a + e0 + E - 1) / E, per = (chunks + W - 1) / W;
     const int lo = part * per, hi = min(chunks, lo + per);
     if (MASK == SB_MASK_NONE) {
-        for (int ch = lo + lane; ch < hi; ch += 32) {
-            const int first = ch * E - e0;
-            const uint32_t head = first < 0 ? ALL << -first : ALL;
-            const uint32_t tail = first + E > a ? ALL >> (32 - (a - first)) : ALL;
-            grad_chunk<T, ENT>(x, g, first, a, head & tail & ((1u << E) - 1u), r, inv_t);
-        }
+        for (int ch = lo + lane; ch < hi; ch += 32) grad_dense<T, ENT>(x, g, ch * E - e0, a, r, inv_t);
     } else {
+        uint32_t* list = reinterpret_cast<uint32_t*>(sh);
+        T* xs = reinterpret_cast<T*>(sh + 4 * CHUNKS + lane * SLOT);
+        T* gs = reinterpret_cast<T*>(sh + 4 * CHUNKS + (32 + lane) * SLOT);
         Chunk<T> zero;
         zero.fill(0);
         int count = 0;
@@ -573,7 +698,7 @@ __device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, con
                 __syncwarp();
                 for (int i = lane; i < count; i += 32) {
                     const uint32_t v = list[i];
-                    grad_chunk<T, ENT>(x, g, (int)(v & 0xffffu) * E - e0, a, v >> 16, r, inv_t);
+                    grad_sparse<T, ENT>(x, g, (int)(v & 0xffffu) * E - e0, a, v >> 16, r, inv_t, xs, gs);
                 }
                 __syncwarp();
                 count = 0;
@@ -591,7 +716,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
     uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
     const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
     uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint32_t* list = reinterpret_cast<uint32_t*>(sh + (WARPS / W) * row_bytes) + warp * CHUNKS;
+    uint8_t* work = sh + (WARPS / W) * row_bytes + warp * GRAD_BYTES;
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
@@ -623,7 +748,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
         if (MASK != SB_MASK_NONE) legal = legal && bits.test((int)act);
         const float total = warp_sum(add) + (legal ? ga : 0.f);
         const RowGrad r = {st.x, st.y, -(total + gh * h), -gh, -(total + gh * h)};
-        const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, list, W == 1 ? 0 : warp);
+        const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
         const bool same = legal && mine == (int)act;
         if (same) add += ga;
         if (mine >= own.x && mine < own.y) out[mine] = from_f<T>(grad_of<true>(to_f(x[mine]), r, r.l0, add, R.inv_t));
@@ -650,11 +775,18 @@ __device__ __forceinline__ int teacher(const Rows& R, const sb_distill& d, Bits 
     return (int)a;
 }
 
+// Loss: one pass for the row's (M, Z), then the teacher's entries by one warp.
+// With the tail, the unlisted actions' own mass p_r is 1 - sum p while that
+// keeps its digits (sum p < 1/2), nothing where every legal action is listed,
+// and otherwise summed by a second pass that leaves the listed ones out.
 template <typename T, int MASK, int W, bool TAIL>
 __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill d) {
     extern __shared__ uint4 dyn[];
     __shared__ Sum sums[WARPS];
+    __shared__ int counts[WARPS];
+    __shared__ int again;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = W == 1 ? lane : threadIdx.x;
+    const int part = W == 1 ? 0 : warp;
     uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
     const int row_bytes = bits_bytes(R.a) * ((MASK != SB_MASK_NONE) + TAIL);
     uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
@@ -671,89 +803,99 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
         if (W == 1) __syncwarp();
         else __syncthreads();
         const Bits skip = {sh_skip, bits.p};
-        // the teacher's weights, and which entry is an action's first
-        Sum ts = no_sum();
-        float sq = 0.f;
-        unsigned first = 0;  // bit j: this lane's entry of round j
+        Sum s = no_sum();
+        Top none;
+        int legal = 0;
+        if (MASK == SB_MASK_NONE) pass_all<T, W, false, false>(s, x, skip, R.a, c, part);
+        else legal = pass_masked<T, W, false, false, false>(s, none, x, bits, bits, R.a, c, list, part);
+        if (W > 1 && lane == 0) counts[warp] = legal;
+        s = whole<W>(s, c, sums);
+        if (W > 1) {
+            legal = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) legal += counts[w];
+        }
+        if (MASK == SB_MASK_NONE) legal = R.a;
+        const float2 st = stats_of(s);
+        float loss = 0.f, total = 0.f, share = 0.f;
+        float2 tst = make_float2(0.f, 0.f);
+        bool more = false;  // a second pass is needed
         if (W == 1 || warp == 0) {
-            for (int k0 = 0, j = 0; k0 < d.listed; k0 += 32, ++j) {
-                float v = 0.f;
+            if (!TAIL) {
+                Sum ts = no_sum();
+                for (int k0 = 0; k0 < d.listed; k0 += 32) {
+                    float v = 0.f;
+                    const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
+                    const float t[1] = {a >= 0 ? v : NEG_INF};
+                    take<1, false>(ts, t, c);
+                }
+                tst = stats_of(whole<1>(ts, c, nullptr));
+            }
+            float sp = 0.f;
+            int unique = 0;
+            for (int k0 = 0; k0 < d.listed; k0 += 32) {
+                float v = 0.f, p = 0.f;
                 const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-                if (TAIL) {
-                    if (a >= 0) sq += expf(v);
+                if (a >= 0) {
+                    const float lq = (v - tst.x) * tc - tst.y, q = expf(lq), lp = (to_f(x[a]) - st.x) * R.inv_t - st.y;
+                    loss += q > 0.f || q != q ? q * (lq - lp) : 0.f;
+                    total += q;
+                    p = expf(lp);
+                }
+                if (TAIL) {  // an action's first entry stands for it in p
                     const unsigned peers = __match_any_sync(ALL, a);
                     const bool lead = a >= 0 && (peers & ((1u << lane) - 1u)) == 0 && !skip.test(a);
                     __syncwarp();
                     if (lead) {
-                        first |= 1u << j;
+                        sp += p;
                         atomicOr(&sh_skip[(a + skip.p) >> 5], 1u << ((a + skip.p) & 31));
                     }
+                    unique += __popc(__ballot_sync(ALL, lead));
                     __syncwarp();
-                } else {
-                    float t[1] = {a >= 0 ? v : NEG_INF};
-                    take<1, false>(ts, t, c);
-                }
-            }
-        }
-        if (TAIL && W > 1) __syncthreads();
-        Sum s = no_sum();
-        Top none;
-        if (MASK == SB_MASK_NONE) pass_all<T, W, false, false>(s, none, x, TAIL ? &skip : nullptr, R.a, c, W == 1 ? 0 : warp);
-        else pass_masked<T, W, false, false>(s, none, x, bits, TAIL ? sh_skip : nullptr, R.a, c, list, W == 1 ? 0 : warp);
-        s = whole<W>(s, c, sums);
-        if (W == 1 || warp == 0) {
-            Sum all = s, in = no_sum();
-            float2 tst = make_float2(0.f, 0.f);
-            if (TAIL) {
-                sq = warp_sum(sq);
-                for (int k0 = 0, j = 0; k0 < d.listed; k0 += 32, ++j) {
-                    float v = 0.f;
-                    const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-                    float t[1] = {(first >> j) & 1 ? to_f(x[a]) : NEG_INF};
-                    take<1, false>(in, t, c);
-                }
-                in = whole<1>(in, c, nullptr);
-                all = join(in, s, c);
-            } else {
-                tst = stats_of(whole<1>(ts, c, nullptr));
-            }
-            const float2 st = stats_of(all);
-            float loss = 0.f, kept = 0.f;
-            for (int k0 = 0; k0 < d.listed; k0 += 32) {
-                float v = 0.f;
-                const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-                if (a >= 0) {
-                    const float lq = (v - tst.x) * tc - tst.y, q = expf(lq);
-                    loss += q * (lq - ((to_f(x[a]) - st.x) * R.inv_t - st.y));
-                    kept += q;
                 }
             }
             loss = warp_sum(loss);
-            float total = TAIL ? sq : warp_sum(kept), share = 0.f;
+            total = warp_sum(total);
             if (TAIL) {
-                // the unlisted actions as one: q_r log(q_r / p_r), each log from
-                // the side that keeps its digits
-                const float qr = s.m > NEG_INF || s.r != s.r ? fmaxf(0.f, 1.f - sq) : 0.f;
-                if (qr > 0.f) {
-                    const float2 si = stats_of(in), sr = stats_of(s);
-                    const float sp = expf((si.x - st.x) * R.inv_t + si.y - st.y);
-                    const float lpr = in.m == NEG_INF ? 0.f
-                                      : sp < 0.5f     ? log1pf(-sp)
-                                                      : (sr.x - st.x) * R.inv_t + sr.y - st.y;
-                    const float lqr = log1pf(-sq);
+                sp = warp_sum(sp);
+                const float qr = legal > unique ? fmaxf(0.f, 1.f - total) : 0.f;
+                more = qr > 0.f && !(sp < 0.5f);
+                if (qr > 0.f && !more) {
+                    const float lqr = log1pf(-total), lpr = log1pf(-sp);
                     loss += qr * (lqr - lpr);
                     share = expf(lqr - lpr);
                     total += qr;
                 }
             }
-            if (lane == 0) {
-                d.loss[row] = loss;
-                if (d.row_stats) {
-                    float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
-                    o[0] = st;
-                    o[1] = make_float2(total, total - share);
-                    o[2] = tst;
+        }
+        if (TAIL) {
+            if (W > 1) {
+                if (threadIdx.x == 0) again = more;
+                __syncthreads();
+                more = again;
+            }
+            if (more) {
+                Sum rest = no_sum();
+                if (MASK == SB_MASK_NONE) pass_all<T, W, false, true>(rest, x, skip, R.a, c, part);
+                else pass_masked<T, W, false, false, true>(rest, none, x, bits, skip, R.a, c, list, part);
+                rest = whole<W>(rest, c, sums);
+                if ((W == 1 || warp == 0) && rest.m > NEG_INF) {
+                    const float2 sr = stats_of(rest);
+                    const float qr = fmaxf(0.f, 1.f - total), lqr = log1pf(-total);
+                    const float lpr = (sr.x - st.x) * R.inv_t + sr.y - st.y;
+                    loss += qr * (lqr - lpr);
+                    share = expf(lqr - lpr);
+                    total += qr;
                 }
+            }
+        }
+        if ((W == 1 || warp == 0) && lane == 0) {
+            d.loss[row] = loss;
+            if (d.row_stats) {
+                float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
+                o[0] = st;
+                o[1] = make_float2(total, total - share);
+                o[2] = tst;
             }
         }
         if (W > 1) __syncthreads();
@@ -769,7 +911,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
     uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
     const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
     uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint32_t* list = reinterpret_cast<uint32_t*>(sh + (WARPS / W) * row_bytes) + warp * CHUNKS;
+    uint8_t* work = sh + (WARPS / W) * row_bytes + warp * GRAD_BYTES;
     const float tc = d.tail ? 1.f : R.inv_t;
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
@@ -785,7 +927,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
             else __syncthreads();
         }
         const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
-        const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, list, W == 1 ? 0 : warp);
+        const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
         for (int k0 = 0; k0 < d.listed; k0 += 32) {
             float v = 0.f;
             const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
@@ -844,11 +986,9 @@ unsigned grid_of(int64_t rows, int w) {
 
 template <int V> using Const = std::integral_constant<int, V>;
 
-// Call f(element type, mask kind, warps per row) as constants: four warps
-// where one would have more than ROW_BYTES to stream for a row.
+// Call f(element type, mask kind, warps per row) as constants.
 template <typename F>
-int dispatch(const sb_logits* x, int64_t bytes, F f) {
-    const bool wide = bytes > ROW_BYTES;
+int dispatch(const sb_logits* x, bool wide, F f) {
     auto kinds = [&](auto* t) {
         switch (x->mask_kind) {
             case SB_MASK_U8: return wide ? f(t, Const<SB_MASK_U8>{}, Const<WARPS>{}) : f(t, Const<SB_MASK_U8>{}, Const<1>{});
@@ -864,11 +1004,15 @@ int dispatch(const sb_logits* x, int64_t bytes, F f) {
 
 int64_t row_bytes(const sb_logits* x) { return (int64_t)x->n_actions * (x->dtype == SB_DTYPE_F32 ? 4 : 2); }
 
-// What a forward pass streams of a row whatever it holds.
-int64_t read_bytes(const sb_logits* x) {
-    if (x->mask_kind == SB_MASK_U8) return x->n_actions;
-    return x->mask_kind == SB_MASK_BITS ? (x->n_actions + 7) / 8 : row_bytes(x);
+// Four warps per row where one would have a long chain of loads for it: more
+// than 4 KB of an unmasked row (32 elements a lane and turn), a mask of more
+// than 16,384 actions (2 KB of staged bits a warp), or a masked gradient row
+// of more than 64 KB (1 KB of zeros a turn).  Splitting a shorter masked row
+// costs more than it gives: each warp pays for its own joins.
+bool wide_forward(const sb_logits* x) {
+    return x->mask_kind == SB_MASK_NONE ? row_bytes(x) > 4096 : x->n_actions > 16384;
 }
+bool wide_backward(const sb_logits* x) { return row_bytes(x) > (x->mask_kind == SB_MASK_NONE ? 4096 : 65536); }
 
 int check_logprobs(const sb_logits* x, const sb_logprobs* o) {
     if (!o) return fail(SB_E_ARG, "outputs description is NULL");
@@ -910,7 +1054,7 @@ int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream)
         return fail(SB_E_ARG, "entropy is NULL, or actions and logprob disagree");
     if (out->top && (!out->top_action || !out->top_logprob)) return fail(SB_E_ARG, "top outputs are NULL");
     if (out->row_stats && !aligned(out->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
-    return dispatch(x, read_bytes(x), [&](auto* t, auto mask, auto w) {
+    return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int M = decltype(mask)::value, W = decltype(w)::value;
         const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 2 * LIST;
@@ -933,10 +1077,10 @@ int sb_action_logprobs_backward(const sb_logits* x, const sb_logprobs* fwd, cons
     if (!aligned(fwd->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
     if ((g->g_logprob && !fwd->actions) || (g->g_top && (!fwd->top || !fwd->top_action)))
         return fail(SB_E_ARG, "a gradient of an output that the forward call did not have");
-    return dispatch(x, row_bytes(x), [&](auto* t, auto mask, auto w) {
+    return dispatch(x, wide_backward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 4 * CHUNKS;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * GRAD_BYTES;
         logprobs_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *fwd, *g);
         return launched("logprobs_backward_kernel launch");
     });
@@ -947,7 +1091,7 @@ int sb_distill_loss(const sb_logits* x, const sb_distill* d, void* stream) {
     int rc = check_rows(x, &R);
     if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
     if (!d->loss) return fail(SB_E_ARG, "loss is NULL");
-    return dispatch(x, read_bytes(x), [&](auto* t, auto mask, auto w) {
+    return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int M = decltype(mask)::value, W = decltype(w)::value;
         const int lists = M == SB_MASK_NONE ? 0 : WARPS * 2 * LIST;
@@ -967,10 +1111,10 @@ int sb_distill_loss_backward(const sb_logits* x, const sb_distill* d, const floa
     if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
     if (!g_loss || !grad || !d->row_stats) return fail(SB_E_ARG, "g_loss, grad or row_stats is NULL");
     if (!aligned(grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
-    return dispatch(x, row_bytes(x), [&](auto* t, auto mask, auto w) {
+    return dispatch(x, wide_backward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 4 * CHUNKS;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * GRAD_BYTES;
         distill_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(
             R, *d, g_loss, g_loss_stride, static_cast<T*>(grad));
         return launched("distill_backward_kernel launch");

@@ -10,6 +10,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -20,8 +22,8 @@ LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libstratego_b200.so"
 # the debug build: every kernel checks each game record's indices first (SB_DEBUG_BOUNDS)
 DEBUG_LIB_PATH = LIB_DIR / "libstratego_b200_debug.so"
-SOURCES = [CSRC / "sb_kernels.cu", CSRC / "sb_policy.cu"]
-DEPS = SOURCES + [CSRC / "sb_device.cuh", CSRC / "sb_error.h", INCLUDE / "stratego_b200.h"]
+SOURCES = [CSRC / f for f in ("sb_kernels.cu", "sb_logprobs.cu", "sb_distill.cu", "sb_policy_small.cu")]
+DEPS = SOURCES + [CSRC / "sb_device.cuh", CSRC / "sb_error.h", CSRC / "sb_policy.cuh", INCLUDE / "stratego_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -46,13 +48,20 @@ def up_to_date(path: Path = LIB_PATH) -> bool:
 
 def _compile(path: Path, extra: list[str], verbose: bool) -> None:
     LIB_DIR.mkdir(exist_ok=True)
-    tmp = path.with_name(f".{path.name}.{os.getpid()}.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, *extra, f"-I{INCLUDE}", "-o", str(tmp), *map(str, SOURCES)]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, path)
+    with tempfile.TemporaryDirectory(dir=LIB_DIR) as tmp:
+        cmds, objs = [], []
+        for src in SOURCES:
+            objs.append(str(Path(tmp) / f"{src.stem}.o"))
+            cmds.append([nvcc(), *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS[:-3], *extra, f"-I{INCLUDE}",
+                         "-Xcompiler", "-fPIC", "-c", "-o", objs[-1], str(src)])
+        lib = Path(tmp) / path.name
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds), flush=True)
+        with ThreadPoolExecutor(len(cmds)) as pool:  # one nvcc per source file at a time
+            for done in pool.map(lambda c: subprocess.run(c), cmds):
+                done.check_returncode()
+        subprocess.run([nvcc(), *NVCC_FLAGS, "-o", str(lib), *objs], check=True)
+        os.replace(lib, path)
 
 
 def build(force: bool = False, verbose: bool = False, debug: bool = True) -> Path:

@@ -1,0 +1,185 @@
+// sb_logprobs.cu -- log-probabilities of given actions, entropy and the likeliest
+// alternatives of policy rows, and their gradient.
+#include "sb_policy.cuh"
+
+namespace sb {
+namespace {
+
+// ---- forward: given actions, entropy, top alternatives -----------------------------
+
+template <typename T, int MASK, int W, bool TOP>
+__global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprobs o) {
+    extern __shared__ uint4 dyn[];
+    __shared__ Sum sums[WARPS];
+    __shared__ float top_x[WARPS][32];
+    __shared__ int top_a[WARPS][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
+    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
+    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
+    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
+    const float c = R.inv_t * LOG2E;
+    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
+    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
+        const T* x = static_cast<const T*>(R.x) + row * R.stride;
+        int64_t act = -1;
+        float xa = 0.f;
+        if (o.actions) {
+            act = load_index(o.actions, o.action_bytes, row);
+            if (act >= 0 && act < R.a) xa = to_f(x[act]);
+        }
+        Sum s = no_sum();
+        Top top;
+        top.init(TOP ? o.top : 1);
+        bool legal = act >= 0 && act < R.a;
+        if (MASK == SB_MASK_NONE) {
+            const float best = pass_all<T, W, true, false>(s, x, Bits{}, R.a, c, W == 1 ? 0 : warp);
+            if (TOP) {
+                top_x[warp][lane] = best;
+                if (W == 1) __syncwarp();
+            }
+        } else {
+            const Bits bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            if (W == 1) __syncwarp();
+            else __syncthreads();
+            legal = legal && bits.test((int)act);
+            pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, W == 1 ? 0 : warp);
+        }
+        if (TOP && W > 1 && MASK != SB_MASK_NONE) {
+            top_x[warp][lane] = top.x;
+            top_a[warp][lane] = top.a;
+        }
+        s = whole<W>(s, c, sums);
+        const float2 st = stats_of(s);
+        if (W == 1 || warp == 0) {
+            if (lane == 0) {
+                if (o.logprob) o.logprob[row] = act == -1 ? 0.f : legal ? (xa - st.x) * R.inv_t - st.y : NEG_INF;
+                o.entropy[row] = st.y == INFINITY ? 0.f : st.y - LN2 * s.t / (s.n + s.r);
+                if (o.row_stats) *reinterpret_cast<float2*>(o.row_stats + 2 * row) = st;
+            }
+            if (TOP) {
+                if (MASK == SB_MASK_NONE)
+                    top_of_all<T, W>(top, x, R.a, top_x[W == 1 ? warp : 0]);
+                else if (W > 1)
+                    for (int w = 1; w < W; ++w) top.offer(lane < o.top ? top_x[w][lane] : NEG_INF, top_a[w][lane]);
+                if (lane < o.top) {
+                    const bool some = top.x > NEG_INF;
+                    o.top_action[row * o.top + lane] = some ? top.a : -1;
+                    o.top_logprob[row * o.top + lane] =
+                        st.y != st.y ? NAN : some ? (top.x - st.x) * R.inv_t - st.y : NEG_INF;
+                }
+            }
+        }
+        if (W > 1) __syncthreads();
+        else __syncwarp();
+    }
+}
+
+template <typename T, int MASK, int W>
+__global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, sb_logprobs f, sb_logprobs_grad g) {
+    extern __shared__ uint4 dyn[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
+    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
+    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
+    uint8_t* work = sh + (WARPS / W) * row_bytes + warp * GRAD_BYTES;
+    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
+    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
+        const T* x = static_cast<const T*>(R.x) + row * R.stride;
+        T* out = static_cast<T*>(g.grad) + row * R.a;
+        // lane k < top holds alternative k; the given action's share joins the
+        // alternative that is the same action, or stays alone
+        int mine = -1;
+        float add = 0.f;
+        if (g.g_top && lane < f.top) {
+            mine = (int)f.top_action[row * f.top + lane];
+            if (mine >= 0) add = g.g_top[row * f.top + lane];
+        }
+        int64_t act = -1;
+        float ga = 0.f;
+        if (g.g_logprob) {
+            act = load_index(f.actions, f.action_bytes, row);
+            ga = g.g_logprob[row * g.g_logprob_stride];
+        }
+        const float gh = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] : 0.f;
+        const float2 st = *reinterpret_cast<const float2*>(f.row_stats + 2 * row);
+        const float h = f.entropy[row];
+        Bits bits = {nullptr, 0};
+        if (MASK != SB_MASK_NONE) {
+            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            if (W == 1) __syncwarp();
+            else __syncthreads();
+        }
+        bool legal = act >= 0 && act < R.a;
+        if (MASK != SB_MASK_NONE) legal = legal && bits.test((int)act);
+        const float total = warp_sum(add) + (legal ? ga : 0.f);
+        const RowGrad r = {st.x, st.y, -(total + gh * h), -gh, -(total + gh * h)};
+        const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
+        const bool same = legal && mine == (int)act;
+        if (same) add += ga;
+        if (mine >= own.x && mine < own.y) out[mine] = from_f<T>(grad_of<true>(to_f(x[mine]), r, r.l0, add, R.inv_t));
+        if (!__any_sync(ALL, same) && lane == 0 && legal && act >= own.x && act < own.y)
+            out[act] = from_f<T>(grad_of<true>(to_f(x[act]), r, r.l0, ga, R.inv_t));
+        if (W > 1) __syncthreads();
+        else __syncwarp();
+    }
+}
+
+int check_logprobs(const sb_logits* x, const sb_logprobs* o) {
+    if (!o) return fail(SB_E_ARG, "outputs description is NULL");
+    if (o->top < 0 || o->top > SB_POLICY_MAX_TOP) return fail(SB_E_ARG, "top must be 0..%d", SB_POLICY_MAX_TOP);
+    if (o->actions && !index_bytes_ok(o->action_bytes)) return fail(SB_E_ARG, "actions must be 2, 4 or 8 bytes wide");
+    if (o->actions && !aligned(o->actions, o->action_bytes)) return fail(SB_E_ARG, "actions not aligned to their type");
+    return SB_OK;
+}
+
+}  // namespace
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" {
+
+int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream) {
+    Rows R;
+    int rc = check_rows(x, &R);
+    if (rc != SB_OK || (rc = check_logprobs(x, out)) != SB_OK || x->n_rows == 0) return rc;
+    if (!out->entropy || (out->actions != nullptr) != (out->logprob != nullptr))
+        return fail(SB_E_ARG, "entropy is NULL, or actions and logprob disagree");
+    if (out->top && (!out->top_action || !out->top_logprob)) return fail(SB_E_ARG, "top outputs are NULL");
+    if (out->row_stats && !aligned(out->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
+    if (R.a <= SMALL) return small_logprobs(x, *out, (cudaStream_t)stream);
+    return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 2 * LIST;
+        if (out->top)
+            logprobs_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
+        else
+            logprobs_kernel<T, M, W, false><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
+        return launched("logprobs_kernel launch");
+    });
+}
+
+int sb_action_logprobs_backward(const sb_logits* x, const sb_logprobs* fwd, const sb_logprobs_grad* g, void* stream) {
+    Rows R;
+    int rc = check_rows(x, &R);
+    if (rc != SB_OK || (rc = check_logprobs(x, fwd)) != SB_OK) return rc;
+    if (!g) return fail(SB_E_ARG, "gradient description is NULL");
+    if (x->n_rows == 0) return SB_OK;
+    if (!g->grad || !fwd->row_stats || !fwd->entropy) return fail(SB_E_ARG, "grad, row_stats or entropy is NULL");
+    if (!aligned(g->grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
+    if (!aligned(fwd->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
+    if ((g->g_logprob && !fwd->actions) || (g->g_top && (!fwd->top || !fwd->top_action)))
+        return fail(SB_E_ARG, "a gradient of an output that the forward call did not have");
+    if (R.a <= SMALL) return small_logprobs_backward(x, *fwd, *g, (cudaStream_t)stream);
+    return dispatch(x, wide_backward(x), [&](auto* t, auto mask, auto w) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
+        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * GRAD_BYTES;
+        logprobs_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *fwd, *g);
+        return launched("logprobs_backward_kernel launch");
+    });
+}
+
+}  // extern "C"

@@ -1,6 +1,8 @@
-// sb_policy.cu -- operators on rows of policy logits under a legal-action
-// mask: log-probabilities of given actions with entropy and top alternatives,
-// and the divergence from a teacher's listed actions, both with gradients.
+// sb_policy.cuh -- what the operators on rows of policy logits under a
+// legal-action mask share: log-probabilities of given actions with entropy and
+// top alternatives (sb_logprobs.cu), and the divergence from a teacher's
+// listed actions (sb_distill.cu), both with gradients; rows of up to 128
+// actions have kernels of their own (sb_policy_small.cu).
 //
 // Mathematics, per row with legal set L and temperature T:
 //   M = max_L x, d_a = (x_a - M) / T, Z = sum_L exp(d_a), log p_a = d_a - log Z
@@ -19,6 +21,7 @@
 // staged in shared memory as one bit per action, and only the logits of set
 // bits are read: a position has some 30 legal moves of 10,000, so a row costs
 // its mask and 30 sectors instead of 20 or 40 KB.
+#pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -521,76 +524,6 @@ __device__ __forceinline__ void top_of_all(Top& top, const T* x, int a, const fl
     }
 }
 
-// ---- forward: given actions, entropy, top alternatives -----------------------------
-
-template <typename T, int MASK, int W, bool TOP>
-__global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprobs o) {
-    extern __shared__ uint4 dyn[];
-    __shared__ Sum sums[WARPS];
-    __shared__ float top_x[WARPS][32];
-    __shared__ int top_a[WARPS][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
-    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
-    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
-    const float c = R.inv_t * LOG2E;
-    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
-    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
-        const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        int64_t act = -1;
-        float xa = 0.f;
-        if (o.actions) {
-            act = load_index(o.actions, o.action_bytes, row);
-            if (act >= 0 && act < R.a) xa = to_f(x[act]);
-        }
-        Sum s = no_sum();
-        Top top;
-        top.init(TOP ? o.top : 1);
-        bool legal = act >= 0 && act < R.a;
-        if (MASK == SB_MASK_NONE) {
-            const float best = pass_all<T, W, true, false>(s, x, Bits{}, R.a, c, W == 1 ? 0 : warp);
-            if (TOP) {
-                top_x[warp][lane] = best;
-                if (W == 1) __syncwarp();
-            }
-        } else {
-            const Bits bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
-            if (W == 1) __syncwarp();
-            else __syncthreads();
-            legal = legal && bits.test((int)act);
-            pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, W == 1 ? 0 : warp);
-        }
-        if (TOP && W > 1 && MASK != SB_MASK_NONE) {
-            top_x[warp][lane] = top.x;
-            top_a[warp][lane] = top.a;
-        }
-        s = whole<W>(s, c, sums);
-        const float2 st = stats_of(s);
-        if (W == 1 || warp == 0) {
-            if (lane == 0) {
-                if (o.logprob) o.logprob[row] = act == -1 ? 0.f : legal ? (xa - st.x) * R.inv_t - st.y : NEG_INF;
-                o.entropy[row] = st.y == INFINITY ? 0.f : st.y - LN2 * s.t / (s.n + s.r);
-                if (o.row_stats) *reinterpret_cast<float2*>(o.row_stats + 2 * row) = st;
-            }
-            if (TOP) {
-                if (MASK == SB_MASK_NONE)
-                    top_of_all<T, W>(top, x, R.a, top_x[W == 1 ? warp : 0]);
-                else if (W > 1)
-                    for (int w = 1; w < W; ++w) top.offer(lane < o.top ? top_x[w][lane] : NEG_INF, top_a[w][lane]);
-                if (lane < o.top) {
-                    const bool some = top.x > NEG_INF;
-                    o.top_action[row * o.top + lane] = some ? top.a : -1;
-                    o.top_logprob[row * o.top + lane] =
-                        st.y != st.y ? NAN : some ? (top.x - st.x) * R.inv_t - st.y : NEG_INF;
-                }
-            }
-        }
-        if (W > 1) __syncthreads();
-        else __syncwarp();
-    }
-}
-
 // ---- gradient rows ---------------------------------------------------------------------
 
 // Gradient of a row: p (c0 + c1 log p) / T off the listed actions, and
@@ -709,251 +642,9 @@ __device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, con
     return make_int2(max(0, lo * E - e0), hi * E - e0);
 }
 
-template <typename T, int MASK, int W>
-__global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, sb_logprobs f, sb_logprobs_grad g) {
-    extern __shared__ uint4 dyn[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
-    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
-    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint8_t* work = sh + (WARPS / W) * row_bytes + warp * GRAD_BYTES;
-    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
-    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
-        const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        T* out = static_cast<T*>(g.grad) + row * R.a;
-        // lane k < top holds alternative k; the given action's share joins the
-        // alternative that is the same action, or stays alone
-        int mine = -1;
-        float add = 0.f;
-        if (g.g_top && lane < f.top) {
-            mine = (int)f.top_action[row * f.top + lane];
-            if (mine >= 0) add = g.g_top[row * f.top + lane];
-        }
-        int64_t act = -1;
-        float ga = 0.f;
-        if (g.g_logprob) {
-            act = load_index(f.actions, f.action_bytes, row);
-            ga = g.g_logprob[row * g.g_logprob_stride];
-        }
-        const float gh = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] : 0.f;
-        const float2 st = *reinterpret_cast<const float2*>(f.row_stats + 2 * row);
-        const float h = f.entropy[row];
-        Bits bits = {nullptr, 0};
-        if (MASK != SB_MASK_NONE) {
-            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
-            if (W == 1) __syncwarp();
-            else __syncthreads();
-        }
-        bool legal = act >= 0 && act < R.a;
-        if (MASK != SB_MASK_NONE) legal = legal && bits.test((int)act);
-        const float total = warp_sum(add) + (legal ? ga : 0.f);
-        const RowGrad r = {st.x, st.y, -(total + gh * h), -gh, -(total + gh * h)};
-        const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
-        const bool same = legal && mine == (int)act;
-        if (same) add += ga;
-        if (mine >= own.x && mine < own.y) out[mine] = from_f<T>(grad_of<true>(to_f(x[mine]), r, r.l0, add, R.inv_t));
-        if (!__any_sync(ALL, same) && lane == 0 && legal && act >= own.x && act < own.y)
-            out[act] = from_f<T>(grad_of<true>(to_f(x[act]), r, r.l0, ga, R.inv_t));
-        if (W > 1) __syncthreads();
-        else __syncwarp();
-    }
-}
+// ---- host side -----------------------------------------------------------------------------
 
-// ---- distillation ------------------------------------------------------------------------
-
-// Kept per row for the backward pass: (M, log Z), (Q, Q - q_r / p_r) and the
-// teacher's own (maximum, log sum).
-
-// Teacher entry k of a row: its action (-1 where it is left out) and logit.
-template <int MASK>
-__device__ __forceinline__ int teacher(const Rows& R, const sb_distill& d, Bits bits, int64_t row, int k, float* v) {
-    if (k >= d.listed) return -1;
-    const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
-    *v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
-    if (a < 0 || a >= R.a || *v == NEG_INF) return -1;
-    if (MASK != SB_MASK_NONE && !bits.test((int)a)) return -1;
-    return (int)a;
-}
-
-// Loss: one pass for the row's (M, Z), then the teacher's entries by one warp.
-// With the tail, the unlisted actions' own mass p_r is 1 - sum p while that
-// keeps its digits (sum p < 1/2), nothing where every legal action is listed,
-// and otherwise summed by a second pass that leaves the listed ones out.
-template <typename T, int MASK, int W, bool TAIL>
-__global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill d) {
-    extern __shared__ uint4 dyn[];
-    __shared__ Sum sums[WARPS];
-    __shared__ int counts[WARPS];
-    __shared__ int again;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = W == 1 ? lane : threadIdx.x;
-    const int part = W == 1 ? 0 : warp;
-    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
-    const int row_bytes = bits_bytes(R.a) * ((MASK != SB_MASK_NONE) + TAIL);
-    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint32_t* sh_skip = reinterpret_cast<uint32_t*>(sh_bits + (MASK != SB_MASK_NONE ? bits_bytes(R.a) : 0));
-    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
-    const float c = R.inv_t * LOG2E, tc = TAIL ? 1.f : R.inv_t;
-    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
-    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
-        const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        Bits bits = {nullptr, 0};
-        if (MASK != SB_MASK_NONE) bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, tid);
-        if (TAIL)
-            for (int i = tid; i < bits_bytes(R.a) / 4; i += 32 * W) sh_skip[i] = 0;
-        if (W == 1) __syncwarp();
-        else __syncthreads();
-        const Bits skip = {sh_skip, bits.p};
-        Sum s = no_sum();
-        Top none;
-        int legal = 0;
-        if (MASK == SB_MASK_NONE) pass_all<T, W, false, false>(s, x, skip, R.a, c, part);
-        else legal = pass_masked<T, W, false, false, false>(s, none, x, bits, bits, R.a, c, list, part);
-        if (W > 1 && lane == 0) counts[warp] = legal;
-        s = whole<W>(s, c, sums);
-        if (W > 1) {
-            legal = 0;
-#pragma unroll
-            for (int w = 0; w < W; ++w) legal += counts[w];
-        }
-        if (MASK == SB_MASK_NONE) legal = R.a;
-        const float2 st = stats_of(s);
-        float loss = 0.f, total = 0.f, share = 0.f;
-        float2 tst = make_float2(0.f, 0.f);
-        bool more = false;  // a second pass is needed
-        if (W == 1 || warp == 0) {
-            if (!TAIL) {
-                Sum ts = no_sum();
-                for (int k0 = 0; k0 < d.listed; k0 += 32) {
-                    float v = 0.f;
-                    const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-                    const float t[1] = {a >= 0 ? v : NEG_INF};
-                    take<1, false>(ts, t, c);
-                }
-                tst = stats_of(whole<1>(ts, c, nullptr));
-            }
-            float sp = 0.f;
-            int unique = 0;
-            for (int k0 = 0; k0 < d.listed; k0 += 32) {
-                float v = 0.f, p = 0.f;
-                const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-                if (a >= 0) {
-                    const float lq = (v - tst.x) * tc - tst.y, q = expf(lq), lp = (to_f(x[a]) - st.x) * R.inv_t - st.y;
-                    loss += q > 0.f || q != q ? q * (lq - lp) : 0.f;
-                    total += q;
-                    p = expf(lp);
-                }
-                if (TAIL) {  // an action's first entry stands for it in p
-                    const unsigned peers = __match_any_sync(ALL, a);
-                    const bool lead = a >= 0 && (peers & ((1u << lane) - 1u)) == 0 && !skip.test(a);
-                    __syncwarp();
-                    if (lead) {
-                        sp += p;
-                        atomicOr(&sh_skip[(a + skip.p) >> 5], 1u << ((a + skip.p) & 31));
-                    }
-                    unique += __popc(__ballot_sync(ALL, lead));
-                    __syncwarp();
-                }
-            }
-            loss = warp_sum(loss);
-            total = warp_sum(total);
-            if (TAIL) {
-                sp = warp_sum(sp);
-                const float qr = legal > unique ? fmaxf(0.f, 1.f - total) : 0.f;
-                more = qr > 0.f && !(sp < 0.5f);
-                if (qr > 0.f && !more) {
-                    const float lqr = log1pf(-total), lpr = log1pf(-sp);
-                    loss += qr * (lqr - lpr);
-                    share = expf(lqr - lpr);
-                    total += qr;
-                }
-            }
-        }
-        if (TAIL) {
-            if (W > 1) {
-                if (threadIdx.x == 0) again = more;
-                __syncthreads();
-                more = again;
-            }
-            if (more) {
-                Sum rest = no_sum();
-                if (MASK == SB_MASK_NONE) pass_all<T, W, false, true>(rest, x, skip, R.a, c, part);
-                else pass_masked<T, W, false, false, true>(rest, none, x, bits, skip, R.a, c, list, part);
-                rest = whole<W>(rest, c, sums);
-                if ((W == 1 || warp == 0) && rest.m > NEG_INF) {
-                    const float2 sr = stats_of(rest);
-                    const float qr = fmaxf(0.f, 1.f - total), lqr = log1pf(-total);
-                    const float lpr = (sr.x - st.x) * R.inv_t + sr.y - st.y;
-                    loss += qr * (lqr - lpr);
-                    share = expf(lqr - lpr);
-                    total += qr;
-                }
-            }
-        }
-        if ((W == 1 || warp == 0) && lane == 0) {
-            d.loss[row] = loss;
-            if (d.row_stats) {
-                float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
-                o[0] = st;
-                o[1] = make_float2(total, total - share);
-                o[2] = tst;
-            }
-        }
-        if (W > 1) __syncthreads();
-        else __syncwarp();
-    }
-}
-
-template <typename T, int MASK, int W>
-__global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb_distill d, const float* g_loss,
-                                                                      int64_t g_stride, T* grad) {
-    extern __shared__ uint4 dyn[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
-    const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
-    uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint8_t* work = sh + (WARPS / W) * row_bytes + warp * GRAD_BYTES;
-    const float tc = d.tail ? 1.f : R.inv_t;
-    const int64_t step = (int64_t)gridDim.x * (WARPS / W);
-    for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
-        const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        T* out = grad + row * R.a;
-        const float2* s = reinterpret_cast<const float2*>(d.row_stats + 6 * row);
-        const float2 st = s[0], co = s[1], te = s[2];
-        const float w = g_loss[row * g_stride];
-        Bits bits = {nullptr, 0};
-        if (MASK != SB_MASK_NONE) {
-            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
-            if (W == 1) __syncwarp();
-            else __syncthreads();
-        }
-        const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
-        const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
-        for (int k0 = 0; k0 < d.listed; k0 += 32) {
-            float v = 0.f;
-            const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-            float q = 0.f;
-            // an action that is listed again takes all of its entries' weights:
-            // every one of them stores the same value, summed in the same order
-            for (int j0 = 0; j0 < d.listed; j0 += 32) {
-                float u = 0.f;
-                const int b = j0 == k0 ? a : teacher<MASK>(R, d, bits, row, j0 + lane, &u);
-                if (j0 == k0) u = v;
-                const float qu = b >= 0 ? expf((u - te.x) * tc - te.y) : 0.f;
-                for (int j = 0; j < 32 && j0 + j < d.listed; ++j) {
-                    const int bj = __shfl_sync(ALL, b, j);
-                    const float qj = __shfl_sync(ALL, qu, j);
-                    if (a >= 0 && bj == a) q += qj;
-                }
-            }
-            if (a >= 0 && a >= own.x && a < own.y)
-                out[a] = from_f<T>(grad_of<false>(to_f(x[a]), r, r.l0, -w * q, R.inv_t));
-        }
-        if (W > 1) __syncthreads();
-        else __syncwarp();
-    }
-}
-
-int check_rows(const sb_logits* x, Rows* R) {
+inline int check_rows(const sb_logits* x, Rows* R) {
     if (!x) return fail(SB_E_ARG, "logits description is NULL");
     if (x->n_rows < 0) return fail(SB_E_ARG, "n_rows < 0");
     if (x->n_actions < 1 || x->n_actions > SB_POLICY_MAX_ACTIONS)
@@ -972,14 +663,14 @@ int check_rows(const sb_logits* x, Rows* R) {
     return SB_OK;
 }
 
-bool index_bytes_ok(int b) { return b == 2 || b == 4 || b == 8; }
+inline bool index_bytes_ok(int b) { return b == 2 || b == 4 || b == 8; }
 
-int launched(const char* what) {
+inline int launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? SB_OK : cuda_fail(e, what);
 }
 
-unsigned grid_of(int64_t rows, int w) {
+inline unsigned grid_of(int64_t rows, int w) {
     const int64_t ctas = (rows + WARPS / w - 1) / (WARPS / w);
     return (unsigned)(ctas < 0x7fffffff ? ctas : 0x7fffffff);
 }
@@ -1002,123 +693,26 @@ int dispatch(const sb_logits* x, bool wide, F f) {
     return kinds((__half*)nullptr);
 }
 
-int64_t row_bytes(const sb_logits* x) { return (int64_t)x->n_actions * (x->dtype == SB_DTYPE_F32 ? 4 : 2); }
+inline int64_t row_bytes(const sb_logits* x) { return (int64_t)x->n_actions * (x->dtype == SB_DTYPE_F32 ? 4 : 2); }
 
 // Four warps per row where one would have a long chain of loads for it: more
 // than 4 KB of an unmasked row (32 elements a lane and turn), a mask of more
 // than 16,384 actions (2 KB of staged bits a warp), or a masked gradient row
 // of more than 64 KB (1 KB of zeros a turn).  Splitting a shorter masked row
 // costs more than it gives: each warp pays for its own joins.
-bool wide_forward(const sb_logits* x) {
+inline bool wide_forward(const sb_logits* x) {
     return x->mask_kind == SB_MASK_NONE ? row_bytes(x) > 4096 : x->n_actions > 16384;
 }
-bool wide_backward(const sb_logits* x) { return row_bytes(x) > (x->mask_kind == SB_MASK_NONE ? 4096 : 65536); }
+inline bool wide_backward(const sb_logits* x) { return row_bytes(x) > (x->mask_kind == SB_MASK_NONE ? 4096 : 65536); }
 
-int check_logprobs(const sb_logits* x, const sb_logprobs* o) {
-    if (!o) return fail(SB_E_ARG, "outputs description is NULL");
-    if (o->top < 0 || o->top > SB_POLICY_MAX_TOP) return fail(SB_E_ARG, "top must be 0..%d", SB_POLICY_MAX_TOP);
-    if (o->actions && !index_bytes_ok(o->action_bytes)) return fail(SB_E_ARG, "actions must be 2, 4 or 8 bytes wide");
-    if (o->actions && !aligned(o->actions, o->action_bytes)) return fail(SB_E_ARG, "actions not aligned to their type");
-    return SB_OK;
-}
-
-int check_distill(const sb_logits* x, const sb_distill* d) {
-    if (!d) return fail(SB_E_ARG, "teacher description is NULL");
-    if (d->listed < 1 || d->listed > SB_POLICY_MAX_TEACHER)
-        return fail(SB_E_ARG, "listed must be 1..%d, got %d", SB_POLICY_MAX_TEACHER, d->listed);
-    if (!index_bytes_ok(d->action_bytes)) return fail(SB_E_ARG, "teacher actions must be 2, 4 or 8 bytes wide");
-    if (d->teacher_dtype < SB_DTYPE_F32 || d->teacher_dtype > SB_DTYPE_F16)
-        return fail(SB_E_ARG, "bad teacher dtype %d", d->teacher_dtype);
-    if (d->tail != 0 && d->tail != 1) return fail(SB_E_ARG, "tail must be 0 or 1");
-    if (x->n_rows == 0) return SB_OK;
-    if (!d->teacher_actions || !d->teacher_logits) return fail(SB_E_ARG, "teacher actions or logits are NULL");
-    if (!aligned(d->teacher_actions, d->action_bytes) ||
-        !aligned(d->teacher_logits, d->teacher_dtype == SB_DTYPE_F32 ? 4 : 2))
-        return fail(SB_E_ARG, "teacher actions or logits not aligned to their type");
-    if (d->row_stats && !aligned(d->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
-    return SB_OK;
-}
-
+// Rows of up to SMALL actions: sb_policy_small.cu.
 }  // namespace
+
+constexpr int SMALL = 128;
+int small_logprobs(const sb_logits* x, const sb_logprobs& o, cudaStream_t st);
+int small_logprobs_backward(const sb_logits* x, const sb_logprobs& f, const sb_logprobs_grad& g, cudaStream_t st);
+int small_distill(const sb_logits* x, const sb_distill& d, cudaStream_t st);
+int small_distill_backward(const sb_logits* x, const sb_distill& d, const float* g_loss, int64_t g_stride, void* grad,
+                           cudaStream_t st);
+
 }  // namespace sb
-
-using namespace sb;
-
-extern "C" {
-
-int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream) {
-    Rows R;
-    int rc = check_rows(x, &R);
-    if (rc != SB_OK || (rc = check_logprobs(x, out)) != SB_OK || x->n_rows == 0) return rc;
-    if (!out->entropy || (out->actions != nullptr) != (out->logprob != nullptr))
-        return fail(SB_E_ARG, "entropy is NULL, or actions and logprob disagree");
-    if (out->top && (!out->top_action || !out->top_logprob)) return fail(SB_E_ARG, "top outputs are NULL");
-    if (out->row_stats && !aligned(out->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
-    return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 2 * LIST;
-        if (out->top)
-            logprobs_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
-        else
-            logprobs_kernel<T, M, W, false><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
-        return launched("logprobs_kernel launch");
-    });
-}
-
-int sb_action_logprobs_backward(const sb_logits* x, const sb_logprobs* fwd, const sb_logprobs_grad* g, void* stream) {
-    Rows R;
-    int rc = check_rows(x, &R);
-    if (rc != SB_OK || (rc = check_logprobs(x, fwd)) != SB_OK) return rc;
-    if (!g) return fail(SB_E_ARG, "gradient description is NULL");
-    if (x->n_rows == 0) return SB_OK;
-    if (!g->grad || !fwd->row_stats || !fwd->entropy) return fail(SB_E_ARG, "grad, row_stats or entropy is NULL");
-    if (!aligned(g->grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
-    if (!aligned(fwd->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
-    if ((g->g_logprob && !fwd->actions) || (g->g_top && (!fwd->top || !fwd->top_action)))
-        return fail(SB_E_ARG, "a gradient of an output that the forward call did not have");
-    return dispatch(x, wide_backward(x), [&](auto* t, auto mask, auto w) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * GRAD_BYTES;
-        logprobs_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *fwd, *g);
-        return launched("logprobs_backward_kernel launch");
-    });
-}
-
-int sb_distill_loss(const sb_logits* x, const sb_distill* d, void* stream) {
-    Rows R;
-    int rc = check_rows(x, &R);
-    if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
-    if (!d->loss) return fail(SB_E_ARG, "loss is NULL");
-    return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int lists = M == SB_MASK_NONE ? 0 : WARPS * 2 * LIST;
-        const int smem = WARPS / W * bits_bytes(R.a) * ((M != SB_MASK_NONE) + d->tail) + lists;
-        if (d->tail)
-            distill_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *d);
-        else
-            distill_kernel<T, M, W, false><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *d);
-        return launched("distill_kernel launch");
-    });
-}
-
-int sb_distill_loss_backward(const sb_logits* x, const sb_distill* d, const float* g_loss, int64_t g_loss_stride,
-                             void* grad, void* stream) {
-    Rows R;
-    int rc = check_rows(x, &R);
-    if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
-    if (!g_loss || !grad || !d->row_stats) return fail(SB_E_ARG, "g_loss, grad or row_stats is NULL");
-    if (!aligned(grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
-    return dispatch(x, wide_backward(x), [&](auto* t, auto mask, auto w) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * GRAD_BYTES;
-        distill_backward_kernel<T, M, W><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(
-            R, *d, g_loss, g_loss_stride, static_cast<T*>(grad));
-        return launched("distill_backward_kernel launch");
-    });
-}
-
-}  // extern "C"

@@ -59,11 +59,14 @@ class ActionLogProbs:
 
 def _call(name: str, dev: torch.device, *args) -> None:
     """The library's entry point ``name`` on the current stream of ``dev``."""
-    if torch.cuda.current_device() != dev.index:
+    index = dev.index
+    if torch.cuda.current_device() != index:
         with torch.cuda.device(dev):
-            C.call(name, *args, _raw_stream(dev.index))
+            rc = getattr(C.lib(), name)(*args, _raw_stream(index))
     else:
-        C.call(name, *args, _raw_stream(dev.index))
+        rc = getattr(C.lib(), name)(*args, _raw_stream(index))
+    if rc:
+        C.check(rc)
 
 
 def _check_logits(logits: torch.Tensor, temperature: float) -> None:
@@ -145,46 +148,70 @@ def _row_grad(g: torch.Tensor | None) -> tuple[torch.Tensor | None, int]:
     return g, g.stride(0)
 
 
-def _logprobs_forward(x, mask, kind, actions, top, temperature, stats):
+def _logprobs_forward(x, x_arg, actions, top, keep):
+    """Launch the forward kernel; returns the outputs and its C description (``keep``: with the backward's rows)."""
     r, dev = x.shape[0], x.device
     entropy = torch.empty(r, dtype=torch.float32, device=dev)
     logprob = None if actions is None else torch.empty_like(entropy)
-    row_stats = torch.empty((r, 2), dtype=torch.float32, device=dev) if stats else None
-    top_lp = torch.empty((r, top), dtype=torch.float32, device=dev) if top else None
-    top_action = torch.empty((r, top), dtype=torch.int64, device=dev) if top else None
+    stats = torch.empty((r, 2), dtype=torch.float32, device=dev) if keep else None
+    top_lp = top_action = None
+    if top:
+        top_lp = torch.empty((r, top), dtype=torch.float32, device=dev)
+        top_action = torch.empty((r, top), dtype=torch.int64, device=dev)
+    arg = C.SbLogprobs(_vp(actions), 0 if actions is None else actions.element_size(), top, _vp(logprob),
+                       entropy.data_ptr(), _vp(stats), _vp(top_action), _vp(top_lp))
     if r:
-        out = C.SbLogprobs(_vp(actions), 0 if actions is None else actions.element_size(), top, _vp(logprob),
-                           entropy.data_ptr(), _vp(row_stats), _vp(top_action), _vp(top_lp))
-        _call("sb_action_logprobs", dev, _logits_arg(x, mask, kind, temperature), out)
-    return logprob, entropy, top_lp, top_action, row_stats
+        _call("sb_action_logprobs", dev, x_arg, arg)
+    return logprob, entropy, top_lp, top_action, stats, arg
+
+
+def _first_order(backward):
+    """A backward pass without a derivative of its own: autograd's guard against
+    differentiating it again costs microseconds, so it is put up only where a
+    second derivative could be asked for (``create_graph=True``)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
+def _repoint(x_arg: C.SbLogits, x: torch.Tensor, mask: torch.Tensor | None) -> C.SbLogits:
+    """The description of the forward call for the saved tensors (saved-tensor hooks may have moved them)."""
+    x_arg.logits, x_arg.row_stride = x.data_ptr(), x.stride(0)
+    if mask is not None:
+        x_arg.mask, x_arg.mask_stride = mask.data_ptr(), mask.stride(0)
+    return x_arg
 
 
 class _ActionLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, mask, kind, actions, top, temperature):
-        lp, ent, top_lp, top_action, stats = _logprobs_forward(x, mask, kind, actions, top, temperature, True)
+    def forward(ctx, x, mask, x_arg, actions, top):
+        lp, ent, top_lp, top_action, stats, arg = _logprobs_forward(x, x_arg, actions, top, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, mask, actions, ent, top_action, stats)
-        ctx.args = (kind, top, temperature)
-        if top_action is not None:
-            ctx.mark_non_differentiable(top_action)
+        ctx.args = (x_arg, arg)
+        if not top:
+            return lp, ent
+        ctx.mark_non_differentiable(top_action)
         return lp, ent, top_lp, top_action
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_ent, g_top, _):
+    @_first_order
+    def backward(ctx, g_lp, g_ent, g_top=None, _=None):
         x, mask, actions, ent, top_action, stats = ctx.saved_tensors
-        kind, top, temperature = ctx.args
+        x_arg, arg = ctx.args
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         if x.shape[0]:
             g_lp, s_lp = _row_grad(g_lp)
             g_ent, s_ent = _row_grad(g_ent)
             g_top = None if g_top is None else g_top.float().contiguous()
-            fwd = C.SbLogprobs(_vp(actions), 0 if actions is None else actions.element_size(), top, None,
-                               ent.data_ptr(), stats.data_ptr(), _vp(top_action), None)
+            arg.actions, arg.entropy, arg.row_stats = _vp(actions), ent.data_ptr(), stats.data_ptr()
+            arg.top_action = _vp(top_action)
             g = C.SbLogprobsGrad(_vp(g_lp), _vp(g_ent), _vp(g_top), s_lp, s_ent, grad.data_ptr())
-            _call("sb_action_logprobs_backward", x.device, _logits_arg(x, mask, kind, temperature), fwd, g)
-        return grad, None, None, None, None, None
+            _call("sb_action_logprobs_backward", x.device, _repoint(x_arg, x, mask), arg, g)
+        return grad, None, None, None, None
 
 
 def action_logprobs(
@@ -220,50 +247,51 @@ def action_logprobs(
         actions = _index_rows(actions, lead, "actions", logits.device)
     _check_cuda(logits)
     x = _rows(logits if logits.dim() > 1 else logits.unsqueeze(0))
-    if torch.is_grad_enabled() and x.requires_grad:
-        lp, ent, top_lp, top_action = _ActionLogProbs.apply(x, m, kind, actions, top, temperature)
+    x_arg = _logits_arg(x, m, kind, temperature)
+    top_lp = top_action = None
+    if not (torch.is_grad_enabled() and x.requires_grad):
+        lp, ent, top_lp, top_action, _, _ = _logprobs_forward(x, x_arg, actions, top, False)
+    elif top:
+        lp, ent, top_lp, top_action = _ActionLogProbs.apply(x, m, x_arg, actions, top)
     else:
-        lp, ent, top_lp, top_action, _ = _logprobs_forward(x, m, kind, actions, top, temperature, False)
+        lp, ent = _ActionLogProbs.apply(x, m, x_arg, actions, 0)
     if len(lead) != 1:
         lp, ent = (None if t is None else t.view(lead) for t in (lp, ent))
         top_lp, top_action = (None if t is None else t.view(*lead, top) for t in (top_lp, top_action))
-    return ActionLogProbs(logprob=lp, entropy=ent, top_action=top_action, top_logprob=top_lp)
+    return ActionLogProbs(lp, ent, top_action, top_lp)
 
 
-def _distill_arg(teacher_actions, teacher_logits, tail, loss, stats) -> C.SbDistill:
-    return C.SbDistill(teacher_actions.data_ptr(), teacher_logits.data_ptr(), teacher_actions.element_size(),
-                       _DTYPES[teacher_logits.dtype], teacher_actions.shape[1], tail, _vp(loss), _vp(stats))
-
-
-def _distill_forward(x, mask, kind, t_act, t_log, temperature, tail, keep):
+def _distill_forward(x, x_arg, t_act, t_log, tail, keep):
     r, dev = x.shape[0], x.device
     loss = torch.empty(r, dtype=torch.float32, device=dev)
     stats = torch.empty((r, 6), dtype=torch.float32, device=dev) if keep else None
+    arg = C.SbDistill(t_act.data_ptr(), t_log.data_ptr(), t_act.element_size(), _DTYPES[t_log.dtype], t_act.shape[1],
+                      tail, loss.data_ptr(), _vp(stats))
     if r:
-        _call("sb_distill_loss", dev, _logits_arg(x, mask, kind, temperature),
-              _distill_arg(t_act, t_log, tail, loss, stats))
-    return loss, stats
+        _call("sb_distill_loss", dev, x_arg, arg)
+    return loss, stats, arg
 
 
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, mask, kind, t_act, t_log, temperature, tail):
-        loss, stats = _distill_forward(x, mask, kind, t_act, t_log, temperature, tail, True)
+    def forward(ctx, x, mask, x_arg, t_act, t_log, tail):
+        loss, stats, arg = _distill_forward(x, x_arg, t_act, t_log, tail, True)
         ctx.save_for_backward(x, mask, t_act, t_log, stats)
-        ctx.args = (kind, temperature, tail)
+        ctx.args = (x_arg, arg)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g_loss):
         x, mask, t_act, t_log, stats = ctx.saved_tensors
-        kind, temperature, tail = ctx.args
+        x_arg, arg = ctx.args
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         if x.shape[0]:
             g_loss, stride = _row_grad(g_loss)
-            _call("sb_distill_loss_backward", x.device, _logits_arg(x, mask, kind, temperature),
-                  _distill_arg(t_act, t_log, tail, None, stats), g_loss.data_ptr(), stride, grad.data_ptr())
-        return grad, None, None, None, None, None, None
+            arg.teacher_actions, arg.teacher_logits, arg.row_stats = t_act.data_ptr(), t_log.data_ptr(), stats.data_ptr()
+            _call("sb_distill_loss_backward", x.device, _repoint(x_arg, x, mask), arg, g_loss.data_ptr(), stride,
+                  grad.data_ptr())
+        return grad, None, None, None, None, None
 
 
 def distill_loss(
@@ -313,11 +341,14 @@ def distill_loss(
     m, kind = _mask_rows(mask, logits)
     _check_cuda(logits)
     x = _rows(logits if logits.dim() > 1 else logits.unsqueeze(0))
-    t_act, t_log = t_act.view(-1, k), teacher_logits.contiguous().view(-1, k)
+    x_arg = _logits_arg(x, m, kind, temperature)
+    t_log = teacher_logits.contiguous()
+    if len(lead) != 1:
+        t_act, t_log = t_act.view(-1, k), t_log.view(-1, k)
     if grad and x.requires_grad:
-        loss = _DistillLoss.apply(x, m, kind, t_act, t_log, temperature, int(tail))
+        loss = _DistillLoss.apply(x, m, x_arg, t_act, t_log, 1 if tail else 0)
     else:
-        loss, _ = _distill_forward(x, m, kind, t_act, t_log, temperature, int(tail), False)
+        loss, _, _ = _distill_forward(x, x_arg, t_act, t_log, 1 if tail else 0, False)
     return loss if len(lead) == 1 else loss.view(lead)
 
 

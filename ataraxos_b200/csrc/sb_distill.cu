@@ -10,15 +10,30 @@ namespace {
 // Kept per row for the backward pass: (M, log Z), (Q, Q - q_r / p_r) and the
 // teacher's own (maximum, log sum).
 
-// Teacher entry k of a row: its action (-1 where it is left out) and logit.
+// This lane's teacher entry of a round of 32: its action (-1 where it is left
+// out), logit and student logit.  Loaded before the mask is known (`load`),
+// so the three loads' latency passes beside the mask's, then checked.
+struct Entry {
+    int a;
+    float v, x;
+};
+template <typename T>
+__device__ __forceinline__ Entry load_entry(const Rows& R, const sb_distill& d, const T* x, int64_t row, int k) {
+    Entry e = {-1, 0.f, 0.f};
+    if (k < d.listed) {
+        const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
+        e.v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
+        if (a >= 0 && a < R.a && !(e.v == NEG_INF)) {
+            e.a = (int)a;
+            e.x = to_f(x[a]);
+        }
+    }
+    return e;
+}
 template <int MASK>
-__device__ __forceinline__ int teacher(const Rows& R, const sb_distill& d, Bits bits, int64_t row, int k, float* v) {
-    if (k >= d.listed) return -1;
-    const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
-    *v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
-    if (a < 0 || a >= R.a || *v == NEG_INF) return -1;
-    if (MASK != SB_MASK_NONE && !bits.test((int)a)) return -1;
-    return (int)a;
+__device__ __forceinline__ Entry check_entry(Entry e, Bits bits) {
+    if (MASK != SB_MASK_NONE && e.a >= 0 && !bits.test(e.a)) e.a = -1;
+    return e;
 }
 
 // Loss: one pass for the row's (M, Z), then the teacher's entries by one warp.
@@ -42,6 +57,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
+        Entry e0 = load_entry(R, d, x, row, lane);
         Bits bits = {nullptr, 0};
         if (MASK != SB_MASK_NONE) bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, tid);
         if (TAIL)
@@ -49,6 +65,8 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
         if (W == 1) __syncwarp();
         else __syncthreads();
         const Bits skip = {sh_skip, bits.p};
+        e0 = check_entry<MASK>(e0, bits);
+        auto entry = [&](int k0) { return k0 ? check_entry<MASK>(load_entry(R, d, x, row, k0 + lane), bits) : e0; };
         Sum s = no_sum();
         Top none;
         int legal = 0;
@@ -70,9 +88,8 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
             if (!TAIL) {
                 Sum ts = no_sum();
                 for (int k0 = 0; k0 < d.listed; k0 += 32) {
-                    float v = 0.f;
-                    const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-                    const float t[1] = {a >= 0 ? v : NEG_INF};
+                    const Entry e = entry(k0);
+                    const float t[1] = {e.a >= 0 ? e.v : NEG_INF};
                     take<1, false>(ts, t, c);
                 }
                 tst = stats_of(whole<1>(ts, c, nullptr));
@@ -80,10 +97,11 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
             float sp = 0.f;
             int unique = 0;
             for (int k0 = 0; k0 < d.listed; k0 += 32) {
-                float v = 0.f, p = 0.f;
-                const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
+                const Entry e = entry(k0);
+                const int a = e.a;
+                float p = 0.f;
                 if (a >= 0) {
-                    const float lq = (v - tst.x) * tc - tst.y, q = expf(lq), lp = (to_f(x[a]) - st.x) * R.inv_t - st.y;
+                    const float lq = (e.v - tst.x) * tc - tst.y, q = expf(lq), lp = (e.x - st.x) * R.inv_t - st.y;
                     loss += q > 0.f || q != q ? q * (lq - lp) : 0.f;
                     total += q;
                     p = expf(lp);
@@ -166,33 +184,36 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
         const float2* s = reinterpret_cast<const float2*>(d.row_stats + 6 * row);
         const float2 st = s[0], co = s[1], te = s[2];
         const float w = g_loss[row * g_stride];
+        Entry e0 = load_entry(R, d, x, row, lane);
         Bits bits = {nullptr, 0};
         if (MASK != SB_MASK_NONE) {
             bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
             if (W == 1) __syncwarp();
             else __syncthreads();
         }
+        e0 = check_entry<MASK>(e0, bits);
         const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
         const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
         for (int k0 = 0; k0 < d.listed; k0 += 32) {
-            float v = 0.f;
-            const int a = teacher<MASK>(R, d, bits, row, k0 + lane, &v);
-            float q = 0.f;
-            // an action that is listed again takes all of its entries' weights:
-            // every one of them stores the same value, summed in the same order
-            for (int j0 = 0; j0 < d.listed; j0 += 32) {
-                float u = 0.f;
-                const int b = j0 == k0 ? a : teacher<MASK>(R, d, bits, row, j0 + lane, &u);
-                if (j0 == k0) u = v;
-                const float qu = b >= 0 ? expf((u - te.x) * tc - te.y) : 0.f;
-                for (int j = 0; j < 32 && j0 + j < d.listed; ++j) {
-                    const int bj = __shfl_sync(ALL, b, j);
-                    const float qj = __shfl_sync(ALL, qu, j);
-                    if (a >= 0 && bj == a) q += qj;
+            const Entry e = k0 ? check_entry<MASK>(load_entry(R, d, x, row, k0 + lane), bits) : e0;
+            float q = e.a >= 0 ? expf((e.v - te.x) * tc - te.y) : 0.f;
+            // An action that is listed again takes all of its entries' weights:
+            // each of its lanes adds them in the entries' order and stores the
+            // same value.
+            const unsigned peers = __match_any_sync(ALL, e.a);
+            if (d.listed > 32 || __any_sync(ALL, e.a >= 0 && (peers & (peers - 1)))) {
+                q = 0.f;
+                for (int j0 = 0; j0 < d.listed; j0 += 32) {
+                    const Entry f = j0 == k0 ? e : check_entry<MASK>(load_entry(R, d, x, row, j0 + lane), bits);
+                    const float qf = f.a >= 0 ? expf((f.v - te.x) * tc - te.y) : 0.f;
+                    for (int j = 0; j < 32 && j0 + j < d.listed; ++j) {
+                        const int b = __shfl_sync(ALL, f.a, j);
+                        const float qb = __shfl_sync(ALL, qf, j);
+                        if (b == e.a) q += qb;
+                    }
                 }
             }
-            if (a >= 0 && a >= own.x && a < own.y)
-                out[a] = from_f<T>(grad_of<false>(to_f(x[a]), r, r.l0, -w * q, R.inv_t));
+            if (e.a >= own.x && e.a < own.y) out[e.a] = from_f<T>(grad_of<false>(e.x, r, r.l0, -w * q, R.inv_t));
         }
         if (W > 1) __syncthreads();
         else __syncwarp();

@@ -101,6 +101,8 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
             act = load_index(f.actions, f.action_bytes, row);
             ga = g.g_logprob[row * g.g_logprob_stride];
         }
+        const float xm = mine >= 0 ? to_f(x[mine]) : 0.f;
+        const float xa = act >= 0 && act < R.a ? to_f(x[act]) : 0.f;
         const float gh = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] : 0.f;
         const float2 st = *reinterpret_cast<const float2*>(f.row_stats + 2 * row);
         const float h = f.entropy[row];
@@ -117,9 +119,9 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
         const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
         const bool same = legal && mine == (int)act;
         if (same) add += ga;
-        if (mine >= own.x && mine < own.y) out[mine] = from_f<T>(grad_of<true>(to_f(x[mine]), r, r.l0, add, R.inv_t));
+        if (mine >= own.x && mine < own.y) out[mine] = from_f<T>(grad_of<true>(xm, r, r.l0, add, R.inv_t));
         if (!__any_sync(ALL, same) && lane == 0 && legal && act >= own.x && act < own.y)
-            out[act] = from_f<T>(grad_of<true>(to_f(x[act]), r, r.l0, ga, R.inv_t));
+            out[act] = from_f<T>(grad_of<true>(xa, r, r.l0, ga, R.inv_t));
         if (W > 1) __syncthreads();
         else __syncwarp();
     }

@@ -182,13 +182,19 @@ __device__ __forceinline__ Bits stage(uint8_t* sh, const uint8_t* m, int a, int 
     uint16_t* s2 = reinterpret_cast<uint16_t*>(sh);
     const int lead = 2 + (h > 0), nb = a > h ? (a - h) >> 4 : 0;
     const uint4* g4 = reinterpret_cast<const uint4*>(m + h);
-#pragma unroll 5
-    for (int j = tid; j < nb; j += G) {
-        const uint4 v = __ldg(g4 + j);
-        uint32_t b = 0;
-        if (v.x | v.y | v.z | v.w)
-            b = nonzero_bytes(v.x) | nonzero_bytes(v.y) << 4 | nonzero_bytes(v.z) << 8 | nonzero_bytes(v.w) << 12;
-        s2[lead + j] = (uint16_t)b;
+    constexpr int U = 10;  // loads in flight: a row of 10,000 bytes is two turns of a warp
+    for (int j0 = tid; j0 < nb; j0 += U * G) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = j0 + u * G < nb ? __ldg(g4 + j0 + u * G) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint32_t b = 0;
+            if (v[u].x | v[u].y | v[u].z | v[u].w)
+                b = nonzero_bytes(v[u].x) | nonzero_bytes(v[u].y) << 4 | nonzero_bytes(v[u].z) << 8 |
+                    nonzero_bytes(v[u].w) << 12;
+            if (j0 + u * G < nb) s2[lead + j0 + u * G] = (uint16_t)b;
+        }
     }
     if (tid < 32) {
         const int i = tid < 16 ? tid - off : h + 16 * nb + tid - 16;

@@ -52,16 +52,21 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
     const int row_bytes = bits_bytes(R.a) * ((MASK != SB_MASK_NONE) + TAIL);
     uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
     uint32_t* sh_skip = reinterpret_cast<uint32_t*>(sh_bits + (MASK != SB_MASK_NONE ? bits_bytes(R.a) : 0));
-    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
+    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes + warp * PASS_BYTES);
     const float c = R.inv_t * LOG2E, tc = TAIL ? 1.f : R.inv_t;
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
         Entry e0 = load_entry(R, d, x, row, lane);
         Bits bits = {nullptr, 0};
-        if (MASK != SB_MASK_NONE) bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, tid);
-        if (TAIL)
+        if (MASK != SB_MASK_NONE) bits = stage<MASK, 32 * W>(sh_bits, R, row, tid);
+        // which actions are listed, as bits: needed at once to find an entry's
+        // action in an earlier round, else only for a second pass
+        const bool rounds = TAIL && d.listed > 32;
+        auto clear = [&] {
             for (int i = tid; i < bits_bytes(R.a) / 4; i += 32 * W) sh_skip[i] = 0;
+        };
+        if (rounds) clear();
         if (W == 1) __syncwarp();
         else __syncthreads();
         const Bits skip = {sh_skip, bits.p};
@@ -70,11 +75,12 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
         Sum s = no_sum();
         Top none;
         int legal = 0;
-        if (MASK == SB_MASK_NONE) pass_all<T, W, false, false>(s, x, skip, R.a, c, part);
+        if (MASK == SB_MASK_NONE)
+            s = whole_all<T, W, false>(pass_all<T, W, false, false>(x, skip, R.a, c, part), x, R.a, c, part, sums);
         else legal = pass_masked<T, W, false, false, false>(s, none, x, bits, bits, R.a, c, list, part);
-        if (W > 1 && lane == 0) counts[warp] = legal;
-        s = whole<W>(s, c, sums);
-        if (W > 1) {
+        if (W > 1 && MASK != SB_MASK_NONE && lane == 0) counts[warp] = legal;
+        if (MASK != SB_MASK_NONE) s = whole<W>(s, c, sums);
+        if (W > 1 && MASK != SB_MASK_NONE) {
             legal = 0;
 #pragma unroll
             for (int w = 0; w < W; ++w) legal += counts[w];
@@ -84,6 +90,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
         float loss = 0.f, total = 0.f, share = 0.f;
         float2 tst = make_float2(0.f, 0.f);
         bool more = false;  // a second pass is needed
+        bool lead0 = false;  // entry e0 is its action's first
         if (W == 1 || warp == 0) {
             if (!TAIL) {
                 Sum ts = no_sum();
@@ -108,14 +115,16 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
                 }
                 if (TAIL) {  // an action's first entry stands for it in p
                     const unsigned peers = __match_any_sync(ALL, a);
-                    const bool lead = a >= 0 && (peers & ((1u << lane) - 1u)) == 0 && !skip.test(a);
-                    __syncwarp();
-                    if (lead) {
-                        sp += p;
-                        atomicOr(&sh_skip[(a + skip.p) >> 5], 1u << ((a + skip.p) & 31));
+                    bool lead = a >= 0 && (peers & ((1u << lane) - 1u)) == 0;
+                    if (rounds) {
+                        lead = lead && !skip.test(a);
+                        __syncwarp();
+                        if (lead) atomicOr(&sh_skip[(a + skip.p) >> 5], 1u << ((a + skip.p) & 31));
+                        __syncwarp();
                     }
+                    if (lead) sp += p;
+                    if (k0 == 0) lead0 = lead;
                     unique += __popc(__ballot_sync(ALL, lead));
-                    __syncwarp();
                 }
             }
             loss = warp_sum(loss);
@@ -139,10 +148,21 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
                 more = again;
             }
             if (more) {
+                if (!rounds) {
+                    clear();
+                    if (W == 1) __syncwarp();
+                    else __syncthreads();
+                    if (lead0) atomicOr(&sh_skip[(e0.a + skip.p) >> 5], 1u << ((e0.a + skip.p) & 31));
+                    if (W == 1) __syncwarp();
+                    else __syncthreads();
+                }
                 Sum rest = no_sum();
-                if (MASK == SB_MASK_NONE) pass_all<T, W, false, true>(rest, x, skip, R.a, c, part);
-                else pass_masked<T, W, false, false, true>(rest, none, x, bits, skip, R.a, c, list, part);
-                rest = whole<W>(rest, c, sums);
+                if (MASK == SB_MASK_NONE) {
+                    rest = whole_all<T, W, false>(pass_all<T, W, false, true>(x, skip, R.a, c, part), x, R.a, c, part, sums);
+                } else {
+                    pass_masked<T, W, false, false, true>(rest, none, x, bits, skip, R.a, c, list, part);
+                    rest = whole<W>(rest, c, sums);
+                }
                 if ((W == 1 || warp == 0) && rest.m > NEG_INF) {
                     const float2 sr = stats_of(rest);
                     const float qr = fmaxf(0.f, 1.f - total), lqr = log1pf(-total);
@@ -187,7 +207,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
         Entry e0 = load_entry(R, d, x, row, lane);
         Bits bits = {nullptr, 0};
         if (MASK != SB_MASK_NONE) {
-            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            bits = stage<MASK, 32 * W>(sh_bits, R, row, W == 1 ? lane : threadIdx.x);
             if (W == 1) __syncwarp();
             else __syncthreads();
         }
@@ -253,7 +273,7 @@ int sb_distill_loss(const sb_logits* x, const sb_distill* d, void* stream) {
     return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int lists = M == SB_MASK_NONE ? 0 : WARPS * 2 * LIST;
+        const int lists = M == SB_MASK_NONE ? 0 : WARPS * PASS_BYTES;
         const int smem = WARPS / W * bits_bytes(R.a) * ((M != SB_MASK_NONE) + d->tail) + lists;
         if (d->tail)
             distill_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *d);

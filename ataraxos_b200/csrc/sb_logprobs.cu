@@ -13,11 +13,13 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
     __shared__ Sum sums[WARPS];
     __shared__ float top_x[WARPS][32];
     __shared__ int top_a[WARPS][32];
+    __shared__ int counts[WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part = W == 1 ? 0 : warp;
     uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
     const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
     uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
-    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes) + warp * LIST;
+    uint16_t* list = reinterpret_cast<uint16_t*>(sh + (WARPS / W) * row_bytes + warp * PASS_BYTES);
     const float c = R.inv_t * LOG2E;
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
@@ -33,23 +35,24 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
         top.init(TOP ? o.top : 1);
         bool legal = act >= 0 && act < R.a;
         if (MASK == SB_MASK_NONE) {
-            const float best = pass_all<T, W, true, false>(s, x, Bits{}, R.a, c, W == 1 ? 0 : warp);
-            if (TOP) {
-                top_x[warp][lane] = best;
-                if (W == 1) __syncwarp();
-            }
+            const LaneSum z = pass_all<T, W, true, false>(x, Bits{}, R.a, c, part);
+            if (TOP)
+                top_of_all<T, W>(top, z.m, x, R.a, part, reinterpret_cast<uint64_t*>(sh) + warp * CANDIDATES,
+                                 &counts[warp]);
+            s = whole_all<T, W, true>(z, x, R.a, c, part, sums);
         } else {
-            const Bits bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            const Bits bits = stage<MASK, 32 * W>(sh_bits, R, row, W == 1 ? lane : threadIdx.x);
             if (W == 1) __syncwarp();
             else __syncthreads();
             legal = legal && bits.test((int)act);
-            pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, W == 1 ? 0 : warp);
+            pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, part);
         }
-        if (TOP && W > 1 && MASK != SB_MASK_NONE) {
+        if (TOP && W > 1) {
             top_x[warp][lane] = top.x;
             top_a[warp][lane] = top.a;
         }
-        s = whole<W>(s, c, sums);
+        if (MASK != SB_MASK_NONE) s = whole<W>(s, c, sums);
+        else if (TOP && W > 1) __syncthreads();
         const float2 st = stats_of(s);
         if (W == 1 || warp == 0) {
             if (lane == 0) {
@@ -58,9 +61,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
                 if (o.row_stats) *reinterpret_cast<float2*>(o.row_stats + 2 * row) = st;
             }
             if (TOP) {
-                if (MASK == SB_MASK_NONE)
-                    top_of_all<T, W>(top, x, R.a, top_x[W == 1 ? warp : 0]);
-                else if (W > 1)
+                if (W > 1)
                     for (int w = 1; w < W; ++w) top.offer(lane < o.top ? top_x[w][lane] : NEG_INF, top_a[w][lane]);
                 if (lane < o.top) {
                     const bool some = top.x > NEG_INF;
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
         const float h = f.entropy[row];
         Bits bits = {nullptr, 0};
         if (MASK != SB_MASK_NONE) {
-            bits = stage<MASK, 32 * W>(sh_bits, R.mask + row * R.mask_stride, R.a, W == 1 ? lane : threadIdx.x);
+            bits = stage<MASK, 32 * W>(sh_bits, R, row, W == 1 ? lane : threadIdx.x);
             if (W == 1) __syncwarp();
             else __syncthreads();
         }
@@ -154,7 +155,9 @@ int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream)
     return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int M = decltype(mask)::value, W = decltype(w)::value;
-        const int smem = M == SB_MASK_NONE ? 0 : WARPS / W * bits_bytes(R.a) + WARPS * 2 * LIST;
+        const int smem = M != SB_MASK_NONE ? WARPS / W * bits_bytes(R.a) + WARPS * PASS_BYTES
+                         : out->top        ? WARPS * 8 * CANDIDATES
+                                           : 0;
         if (out->top)
             logprobs_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
         else

@@ -27,6 +27,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <string.h>
 
 #include <type_traits>
 
@@ -40,8 +41,9 @@ constexpr int WARPS = 4;                  // warps of a CTA: one row each, or on
 constexpr unsigned ALL = 0xffffffffu;
 constexpr float NEG_INF = -INFINITY;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int LIST = 1024;                // legal actions a warp gathers at once
-constexpr int BLOCK_WORDS = 11;           // mask words of a lane between two gathers (odd: no bank conflicts)
+constexpr int LIST = 1024;                // legal actions a warp lists at once: those of 32 mask words
+constexpr int WORDS = 320;                // mask words a warp looks through at once
+constexpr int PASS_BYTES = 2 * (LIST + WORDS);  // shared memory of a warp's pass over a masked row
 constexpr int CHUNKS = 64;                // gradient chunks a warp lists at once
 constexpr int SLOT = 48;                  // bytes between two lanes' chunk slots (32 used)
 
@@ -96,6 +98,7 @@ template <typename T> struct Chunk {
     }
     __device__ __forceinline__ float get(int e) const;
     __device__ __forceinline__ void set(int e, float v);
+    __device__ __forceinline__ float max() const;  // NaN aside
 };
 template <> __device__ __forceinline__ float Chunk<float>::get(int e) const { return __uint_as_float(w[e]); }
 template <> __device__ __forceinline__ void Chunk<float>::set(int e, float v) { w[e] = __float_as_uint(v); }
@@ -107,11 +110,41 @@ template <> __device__ __forceinline__ void Chunk<__nv_bfloat16>::set(int e, flo
     w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | b << 16 : (w[e >> 1] & 0xffff0000u) | b;
 }
 template <> __device__ __forceinline__ float Chunk<__half>::get(int e) const {
-    return __half2float(__ushort_as_half((unsigned short)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu)));
+    __half2 h;
+    memcpy(&h, &w[e >> 1], 4);
+    return e & 1 ? __high2float(h) : __low2float(h);
 }
 template <> __device__ __forceinline__ void Chunk<__half>::set(int e, float v) {
     const uint32_t b = __half_as_ushort(__float2half_rn(v));
     w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | b << 16 : (w[e >> 1] & 0xffff0000u) | b;
+}
+
+template <> __device__ __forceinline__ float Chunk<float>::max() const {
+    float m = get(0);
+#pragma unroll
+    for (int e = 1; e < E; ++e) m = fmaxf(m, get(e));
+    return fmaxf(m, NEG_INF);
+}
+// 16-bit elements are compared two at a time as they are.
+template <> __device__ __forceinline__ float Chunk<__nv_bfloat16>::max() const {
+    __nv_bfloat162 m, v;
+    memcpy(&m, &w[0], 4);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        memcpy(&v, &w[i], 4);
+        m = __hmax2(m, v);
+    }
+    return fmaxf(fmaxf(__low2float(m), __high2float(m)), NEG_INF);
+}
+template <> __device__ __forceinline__ float Chunk<__half>::max() const {
+    __half2 m, v;
+    memcpy(&m, &w[0], 4);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        memcpy(&v, &w[i], 4);
+        m = __hmax2(m, v);
+    }
+    return fmaxf(fmaxf(__low2float(m), __high2float(m)), NEG_INF);
 }
 
 __device__ __forceinline__ int64_t load_index(const void* p, int bytes, int64_t i) {
@@ -128,8 +161,8 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i)
 
 // ---- legal bits in shared memory -------------------------------------------
 
-// Bit a + P of `w` is 1 where action a is legal; words before and after the
-// row are 0, so a field that reaches past either end reads zeros.
+// Bit a + P of `w` is 1 where action a is legal.  Words past the row are 0;
+// bits before it may be anything.
 struct Bits {
     uint32_t* w;
     int p;
@@ -139,15 +172,16 @@ struct Bits {
         const int b = 32 * i + p;
         return __funnelshift_r(w[b >> 5], w[(b >> 5) + 1], b & 31);
     }
-    // `len` <= 16 bits of the actions from a on (a >= -16)
+    // `len` <= 16 bits of the actions from a on (a >= -16; 0 for those below 0)
     __device__ __forceinline__ uint32_t field(int a, int len) const {
         const int b = a + p;
-        return __funnelshift_r(w[b >> 5], w[(b >> 5) + 1], b & 31) & ((1u << len) - 1u);
+        const uint32_t f = __funnelshift_r(w[b >> 5], w[(b >> 5) + 1], b & 31) & ((1u << len) - 1u);
+        return a < 0 ? f & (ALL << -a) : f;
     }
 };
 
 // Bytes of a staged row: the bits, 32 of lead (16 to align a bit-packed row's
-// chunks, 16 of zeros) and zeros past the end.
+// chunks, 16 that a field below action 0 may touch) and zeros past the end.
 __host__ __device__ constexpr int bits_bytes(int a) { return ((a + 7) / 8 + 32 + 48 + 15) / 16 * 16; }
 
 __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t v) {  // bit i: byte i of v is not 0
@@ -157,12 +191,38 @@ __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t v) {  // bit i: byte 
 
 // Stage one row's mask with G threads (tid 0..G-1; the caller synchronises).
 template <int MASK, int G>
-__device__ __forceinline__ Bits stage(uint8_t* sh, const uint8_t* m, int a, int tid) {
-    const int h = (int)(-(intptr_t)m & 15), off = (16 - h) & 15;
+__device__ __forceinline__ Bits stage(uint8_t* sh, const Rows& R, int64_t row, int tid) {
+    const uint8_t* m = R.mask + row * R.mask_stride;
+    const int a = R.a, h = (int)(-(intptr_t)m & 15), off = (16 - h) & 15;
+    if (MASK == SB_MASK_BITS && row > 0 && row < R.n - 1 && R.mask_stride >= (a + 7) >> 3) {
+        // The 16-byte chunks that the row touches, whole: the few bytes of them
+        // that are not the row's belong to the rows beside it (a row here has
+        // more than SMALL actions, 16 bytes).  Row byte i goes
+        // to sh[16 + off + i]; the last chunk is cut off after the last action.
+        const int end = 8 * off + a;  // bits from the first chunk's start
+        const int last = (end - 1) >> 7;
+        uint4* s4 = reinterpret_cast<uint4*>(sh + 16);
+        const uint4* g4 = reinterpret_cast<const uint4*>(m - off);
+#pragma unroll 3
+        for (int j = tid; j < last; j += G) s4[j] = __ldg(g4 + j);
+        if (tid < 2) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (tid == 0) {
+                v = __ldg(g4 + last);
+                const int n = end - 128 * last;  // 1..128 bits stay
+                v.x &= n < 32 ? (1u << n) - 1u : ALL;
+                v.y &= n < 64 ? (n > 32 ? (1u << (n - 32)) - 1u : 0u) : ALL;
+                v.z &= n < 96 ? (n > 64 ? (1u << (n - 64)) - 1u : 0u) : ALL;
+                v.w &= n < 128 ? (n > 96 ? (1u << (n - 96)) - 1u : 0u) : ALL;
+            }
+            s4[last + tid] = v;
+        }
+        return {reinterpret_cast<uint32_t*>(sh), 8 * (16 + off)};
+    }
     if (MASK == SB_MASK_BITS) {
-        // Row byte i goes to sh[16 + off + i], so that the 16-byte chunks of
-        // the row in memory stay 16-byte chunks here.  The row's last byte is
-        // always handled as a tail byte: its bits past the last action drop.
+        // A short row, the first or the last one: the chunks inside the row, and
+        // single bytes at its ends.  The row's last byte is always handled as a
+        // tail byte: its bits past the last action drop.
         const int len = (a + 7) >> 3, nb = len - h > 0 ? (len - h - 1) >> 4 : 0;
         uint4* s4 = reinterpret_cast<uint4*>(sh + 16 + off + h);
         const uint4* g4 = reinterpret_cast<const uint4*>(m + h);
@@ -261,7 +321,7 @@ __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
 // the row's warps by way of shared memory.
 template <int W>
 __device__ __forceinline__ Sum whole(Sum s, float c, Sum* sh) {
-    s.n = warp_sum(s.n);
+    s.n = (float)__reduce_add_sync(ALL, (int)s.n);
     s.r = warp_sum(s.r);
     s.t = warp_sum(s.t);
     if (W > 1) {
@@ -348,186 +408,240 @@ struct Top {
 
 // ---- one pass over a row ------------------------------------------------------------
 
-// The legal logits of this warp's blocks of a row (block b is warp b % W's).
-// The legal actions are listed in ascending order and dealt to the lanes in
-// turn, so the sums' order, and with it every bit of the result, is the same
-// for any kind of mask and wherever its rows lie.  SKIP leaves out the
-// actions of `skip`.  Returns how many actions were taken.
+// The legal logits of this warp's part of a row.  Two steps of compaction, as
+// a position's 30 legal moves lie in some 20 of 313 mask words: the words that
+// are not 0 (by ballots), then the actions of 32 such words, a lane each.  The
+// actions come out in ascending order and are dealt to the lanes in turn, so
+// the sums' order, and with it every bit of the result, is the same for any
+// kind of mask and wherever its rows lie.  SKIP leaves out the actions of
+// `skip`.  Returns how many actions were taken.
 template <typename T, int W, bool ENT, bool TOP, bool SKIP>
 __device__ __forceinline__ int pass_masked(Sum& s, Top& top, const T* x, Bits bits, Bits skip, int a, float c,
                                            uint16_t* list, int part) {
     const int lane = threadIdx.x & 31;
-    const int words = (a + 31) >> 5;
-    auto word = [&](int i) { return i >= words ? 0u : SKIP ? bits.word(i) & ~skip.word(i) : bits.word(i); };
+    const unsigned below = (1u << lane) - 1u;
+    const int words = (a + 31) >> 5, per = (words + W - 1) / W;
+    const int hi = W == 1 ? words : min(words, (part + 1) * per);
+    uint16_t* some = list + LIST;
+    auto word = [&](int i) { return SKIP ? bits.word(i) & ~skip.word(i) : bits.word(i); };
     int taken = 0;
-    for (int w0 = part * 32 * BLOCK_WORDS; w0 < words; w0 += 32 * BLOCK_WORDS * W) {
-        const int mine = w0 + lane * BLOCK_WORDS;
-        uint32_t some = 0;  // bit k: the lane's word k is not 0
-        int count = 0;
+    for (int w0 = part * per; w0 < hi; w0 += WORDS) {
+        int n = 0;
 #pragma unroll
-        for (int k = 0; k < BLOCK_WORDS; ++k) {
-            const uint32_t w = word(mine + k);
-            count += __popc(w);
-            some |= w ? 1u << k : 0u;
+        for (int k = 0; k < WORDS / 32; ++k) {
+            const int i = w0 + 32 * k + lane;
+            const bool on = i < hi && word(i) != 0;
+            const unsigned m = __ballot_sync(ALL, on);
+            if (on) some[n + __popc(m & below)] = (uint16_t)i;
+            n += __popc(m);
         }
-        int at = count;
+        __syncwarp();
+        for (int j = 0; j < n; j += 32) {
+            const int i = j + lane < n ? some[j + lane] : 0;
+            uint32_t w = j + lane < n ? word(i) : 0u;
+            const int count = __popc(w);
+            int at = count;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(ALL, at, o);
-            if (lane >= o) at += v;
-        }
-        const int total = __shfl_sync(ALL, at, 31);
-        if (total == 0) continue;
-        const bool first = taken == 0;
-        taken += total;
-        if (total <= LIST) {
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(ALL, at, o);
+                if (lane >= o) at += v;
+            }
+            const int total = __shfl_sync(ALL, at, 31);
             at -= count;
-            uint32_t w = 0;
-            int base = 0;
-            while (some | w) {  // one action a turn, whichever word it is in
-                if (!w) {
-                    const int i = mine + __ffs(some) - 1;
-                    some &= some - 1;
-                    w = word(i);
-                    base = i * 32;
-                }
-                list[at++] = (uint16_t)(base + __ffs(w) - 1);
+            while (w) {
+                list[at++] = (uint16_t)(32 * i + __ffs(w) - 1);
                 w &= w - 1;
             }
             __syncwarp();
             if (TOP || total <= 32) {
-                for (int i = 0; i < total; i += 32) {
-                    const int b = i + lane < total ? list[i + lane] : 0;
-                    const float v[1] = {i + lane < total ? to_f(x[b]) : NEG_INF};
+                for (int q = 0; q < total; q += 32) {
+                    const int b = q + lane < total ? list[q + lane] : 0;
+                    const float v[1] = {q + lane < total ? to_f(x[b]) : NEG_INF};
                     take<1, ENT>(s, v, c);
                     if (TOP) {
-                        if (first && i == 0) top.fill(v[0], b);
+                        if (taken + q == 0) top.fill(v[0], b);
                         else top.offer(v[0], b);
                     }
                 }
             } else {
-                for (int i = 0; i < total; i += 128) {
+                for (int q0 = 0; q0 < total; q0 += 128) {
                     float v[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const int n = i + q * 32 + lane;
-                        v[q] = n < total ? to_f(x[list[n]]) : NEG_INF;
+                        const int b = q0 + q * 32 + lane;
+                        v[q] = b < total ? to_f(x[list[b]]) : NEG_INF;
                     }
                     take<4, ENT>(s, v, c);
                 }
             }
+            taken += total;
             __syncwarp();
-        } else {
-            // too many for the list: every word's 32 actions in turn, a lane each
-            const int end = min(words, w0 + 32 * BLOCK_WORDS);
-            float best = NEG_INF;
-            for (int i = w0; i < end; i += 8) {
-                float v[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const uint32_t m = i + q < end ? word(i + q) : 0u;
-                    v[q] = (m >> lane) & 1 ? to_f(x[(i + q) * 32 + lane]) : NEG_INF;
-                    best = fmaxf(best, v[q]);
-                }
-                take<8, ENT>(s, v, c);
-            }
-            if (TOP) {
-                // only a lane whose best reaches the k-th best of what the list
-                // holds and of all lanes' bests can hold one of the k best
-                Top bar = top;
-                bar.offer(best, lane);
-                unsigned who = __ballot_sync(ALL, best >= bar.bar_x && best > NEG_INF);
-                for (; who; who &= who - 1) {
-                    const int src = __ffs(who) - 1;
-                    for (int i = w0; i < end; i += 32) {
-                        const int b = (i + lane) * 32 + src;
-                        const uint32_t m = i + lane < end ? word(i + lane) : 0u;
-                        top.offer((m >> src) & 1 ? to_f(x[b]) : NEG_INF, b);
-                    }
-                }
-            }
         }
     }
     return taken;
 }
 
-// The same without a mask: 32-byte chunks of the row at their alignment in
-// memory, the ends that do not fill one by single loads.  Returns the lane's
-// largest logit.
-template <typename T> struct Span {
-    int head, chunks;
-    __device__ __forceinline__ Span(const T* x, int a) {
+// ---- one pass over an unmasked row --------------------------------------------------
+
+// A lane's own sums, with its own largest logit m as the reference (no
+// exchange between lanes until the end): s = sum of exp(d), the maximum's 1
+// included, t as in Sum.
+struct LaneSum {
+    float m, s, t;
+};
+
+// The lane's reference becomes m where that is larger.
+template <bool ENT>
+__device__ __forceinline__ void lane_raise(LaneSum& z, float m, float c) {
+    if (m > z.m) {
+        const float d = (z.m - m) * c, f = exp2_(d);
+        if (ENT) z.t = f * (z.t + z.s * fmaxf(d, -1e4f));
+        z.s *= f;
+        z.m = m;
+    }
+}
+template <bool ENT>
+__device__ __forceinline__ void lane_add(LaneSum& z, float x, float ref, float c) {
+    const float d = (x - ref) * c, e = exp2_(d);
+    z.s += e;
+    if (ENT) z.t = fmaf(e, fmaxf(d, -1e4f), z.t);
+}
+
+// How a warp's part of an unmasked row is dealt out: 32-byte chunks at the
+// row's alignment in memory, chunk `part` * 32 + lane + n * 32 W for lane, and
+// the two ends that do not fill a chunk (fewer than 32 elements) one element a
+// lane of part 0.
+template <typename T, int W> struct Deal {
+    static constexpr int E = Chunk<T>::E;
+    int head, chunks, first, end;  // `end`: the lane's element of the ends, or past the row
+    __device__ __forceinline__ Deal(const T* x, int a, int part) {
+        const int lane = threadIdx.x & 31;
         head = min(a, (int)((-(intptr_t)x & 31) / sizeof(T)));
-        chunks = (a - head) / Chunk<T>::E;
+        chunks = (a - head) / E;
+        first = part * 32 + lane;
+        end = part ? a : lane < head ? lane : chunks * E + lane;
     }
 };
 
-template <typename T, int W, bool ENT, bool SKIP>
-__device__ __forceinline__ float pass_all(Sum& s, const T* x, Bits skip, int a, float c, int part) {
-    constexpr int E = Chunk<T>::E, U = 32 / E;
-    const int lane = threadIdx.x & 31;
-    const Span<T> sp(x, a);
-    float best = NEG_INF;
-    if (part == 0) {  // the ends: fewer than two chunks, one element a lane
-        const int b = lane < sp.head ? lane : sp.chunks * E + lane;
-        const float v[1] = {b < a && !(SKIP && skip.test(b)) ? to_f(x[b]) : NEG_INF};
-        best = fmaxf(best, v[0]);
-        take<1, ENT>(s, v, c);
-    }
-    const T* body = x + sp.head;
-    for (int c0 = part * 32; c0 < sp.chunks; c0 += 32 * U * W) {
-        float v[32];
+// One turn: U chunks of a lane, loaded before the first is used.
+template <typename T, int W, int U, bool ENT, bool SKIP>
+__device__ __forceinline__ void lane_turn(LaneSum& z, const T* body, int i, Bits skip, int head, float c) {
+    constexpr int E = Chunk<T>::E;
+    Chunk<T> q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = c0 + u * 32 * W + lane;
-            Chunk<T> q;
-            if (i < sp.chunks) {
-                q.load(body + i * E);
-                const uint32_t out = SKIP ? skip.field(sp.head + i * E, E) : 0u;
+    for (int u = 0; u < U; ++u) q[u].load(body + (i + u * 32 * W) * E);
+    float m = NEG_INF;
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[u * E + e] = SKIP && (out >> e) & 1 ? NEG_INF : q.get(e);
-            } else {
+    for (int u = 0; u < U; ++u) {
+        if (SKIP) {
+            const uint32_t out = skip.field(head + (i + u * 32 * W) * E, E);
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[u * E + e] = NEG_INF;
-            }
+            for (int e = 0; e < E; ++e)
+                if ((out >> e) & 1) q[u].set(e, NEG_INF);
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) best = fmaxf(best, v[i]);
-        take<32, ENT>(s, v, c);
+        m = fmaxf(m, q[u].max());
     }
-    return best;
+    lane_raise<ENT>(z, m, c);
+    const float ref = z.m == NEG_INF ? 0.f : z.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) lane_add<ENT>(z, q[u].get(e), ref, c);
 }
 
-// The k best of an unmasked row, by one warp: `best[W * 32]` holds every
-// lane's largest logit.  The k-th largest of those bounds the k-th best of the
-// row from below, so only the lanes that reach it are looked through again
-// (about k of them, from cache).
-template <typename T, int W>
-__device__ __forceinline__ void top_of_all(Top& top, const T* x, int a, const float* best) {
-    constexpr int E = Chunk<T>::E;
-    const int lane = threadIdx.x & 31;
-    const Span<T> sp(x, a);
-    Top bar = top;
-    bar.fill(best[lane], lane);
+template <typename T, int W, bool ENT, bool SKIP>
+__device__ __forceinline__ LaneSum pass_all(const T* x, Bits skip, int a, float c, int part) {
+    constexpr int U = sizeof(T) == 4 ? 4 : 2;
+    const Deal<T, W> deal(x, a, part);
+    LaneSum z = {NEG_INF, 0.f, 0.f};
+    const T* body = x + deal.head;
+    const float last = deal.end < a && !(SKIP && skip.test(deal.end)) ? to_f(x[deal.end]) : NEG_INF;
+    int i = deal.first;
+    for (; !SKIP && (i | 31) + (U - 1) * 32 * W < deal.chunks; i += U * 32 * W)  // while all lanes have U
+        lane_turn<T, W, U, ENT, false>(z, body, i, skip, 0, c);
+    for (; i < deal.chunks; i += 32 * W) lane_turn<T, W, 1, ENT, SKIP>(z, body, i, skip, deal.head, c);
+    lane_raise<ENT>(z, last, c);
+    lane_add<ENT>(z, last, z.m == NEG_INF ? 0.f : z.m, c);
+    return z;
+}
+
+// The lanes' sums as the row's.  Where one action holds nearly all of the mass,
+// its lane goes over its own elements once more for the sum of the others.
+template <typename T, int W, bool ENT>
+__device__ __forceinline__ Sum whole_all(LaneSum z, const T* x, int a, float c, int part, Sum* sh) {
+    const float m = warp_max(z.m), d = (z.m - m) * c, f = m == NEG_INF ? 1.f : exp2_(d);
+    const bool top = z.m == m && m > NEG_INF;
+    Sum s = {m, top ? 1.f : 0.f, top ? z.s - 1.f : f * z.s, ENT ? f * (z.t + z.s * fmaxf(d, -1e4f)) : 0.f};
+    Sum r = whole<W>(s, c, sh);
+    if (r.n == 1.f && r.r < 0.015625f) {
+        if (z.m == r.m) {
+            const Deal<T, W> deal(x, a, part);
+            float rest = 0.f;
+            for (int i = deal.first; i < deal.chunks; i += 32 * W) {
+                Chunk<T> q;
+                q.load(x + deal.head + i * Chunk<T>::E);
 #pragma unroll
-    for (int w = 1; w < W; ++w) bar.offer(best[w * 32 + lane], w * 32 + lane);
-    for (int w = 0; w < W; ++w) {
-        const float mine = best[w * 32 + lane];
-        unsigned who = __ballot_sync(ALL, mine >= bar.bar_x && mine > NEG_INF);
-        for (; who; who &= who - 1) {
-            const int src = __ffs(who) - 1;
-            // its chunks are w * 32 + src + n * 32 * W, E elements of each
-            for (int i = lane; __any_sync(ALL, w * 32 + src + i / E * 32 * W < sp.chunks); i += 32) {
-                const int ch = w * 32 + src + i / E * 32 * W, b = sp.head + ch * E + i % E;
-                const float v = ch < sp.chunks ? to_f(x[b]) : NEG_INF;
-                top.offer(v >= bar.bar_x ? v : NEG_INF, b);
+                for (int e = 0; e < Chunk<T>::E; ++e) rest += q.get(e) == r.m ? 0.f : exp2_((q.get(e) - r.m) * c);
             }
-            if (w == 0) {  // and its element of the row's ends
-                const int b = src < sp.head ? src : sp.chunks * E + src;
-                top.offer(lane == 0 && b < a ? to_f(x[b]) : NEG_INF, b);
+            if (deal.end < a && to_f(x[deal.end]) != r.m) rest += exp2_((to_f(x[deal.end]) - r.m) * c);
+            s.r = rest;
+        }
+        if (W > 1) __syncthreads();
+        r = whole<W>(s, c, sh);
+    }
+    return r;
+}
+
+// A warp's k best of its part of an unmasked row.  The k-th largest of the
+// lanes' largest logits bounds the k-th best from below, so only the lanes that
+// reach it look through their elements again (from cache), and of those only
+// what reaches it is put in order.
+constexpr int CANDIDATES = 512;
+template <typename T, int W>
+__device__ __forceinline__ void top_of_all(Top& top, float mine, const T* x, int a, int part, uint64_t* cand, int* count) {
+    const int lane = threadIdx.x & 31;
+    Top bar = top;
+    bar.fill(mine, lane);
+    const float low = fmaxf(bar.bar_x, -3.4028235e38f);  // -inf is never listed
+    if (lane == 0) *count = 0;
+    __syncwarp();
+    const Deal<T, W> deal(x, a, part);
+    auto keep = [&](int b) {
+        const int at = atomicAdd(count, 1);
+        if (at < CANDIDATES) cand[at] = (uint64_t)b << 32 | __float_as_uint(to_f(x[b]));
+    };
+    if (mine >= low) {
+        constexpr int E = Chunk<T>::E;
+        for (int i = deal.first; i < deal.chunks; i += 32 * W) {
+            Chunk<T> q;
+            q.load(x + deal.head + i * E);
+            if (q.max() >= low) {
+                uint32_t hit = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) hit |= q.get(e) >= low ? 1u << e : 0u;
+                for (; hit; hit &= hit - 1) keep(deal.head + i * E + __ffs(hit) - 1);
             }
         }
+        if (deal.end < a && to_f(x[deal.end]) >= low) keep(deal.end);
     }
+    __syncwarp();
+    const int n = *count;
+    if (n <= CANDIDATES) {
+        for (int i = 0; i < n; i += 32) {
+            const uint64_t q = i + lane < n ? cand[i + lane] : 0;
+            const float v = i + lane < n ? __uint_as_float((uint32_t)q) : NEG_INF;
+            if (i == 0) top.fill(v, (int)(q >> 32));
+            else top.offer(v, (int)(q >> 32));
+        }
+    } else {  // a row of equal or sorted logits: every lane's elements in turn
+        const int rounds = (deal.chunks + 32 * W - 1) / (32 * W) * Chunk<T>::E;
+        top.offer(deal.end < a ? to_f(x[deal.end]) : NEG_INF, deal.end);
+        for (int i = 0; i < rounds; ++i) {
+            const int ch = deal.first + i / Chunk<T>::E * 32 * W, b = deal.head + ch * Chunk<T>::E + i % Chunk<T>::E;
+            top.offer(ch < deal.chunks ? to_f(x[b]) : NEG_INF, b);
+        }
+    }
+    __syncwarp();
 }
 
 // ---- gradient rows ---------------------------------------------------------------------

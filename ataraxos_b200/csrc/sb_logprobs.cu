@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
     __shared__ int top_a[WARPS][32];
     __shared__ int counts[WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int part = W == 1 ? 0 : warp;
+    const int part = W == 1 ? 0 : warp, tid = W == 1 ? lane : threadIdx.x;
     uint8_t* sh = reinterpret_cast<uint8_t*>(dyn);
     const int row_bytes = MASK == SB_MASK_NONE ? 0 : bits_bytes(R.a);
     uint8_t* sh_bits = sh + (W == 1 ? warp * row_bytes : 0);
@@ -33,26 +33,41 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
         Sum s = no_sum();
         Top top;
         top.init(TOP ? o.top : 1);
+        bool joined = false;  // the first warp's list is the row's
         bool legal = act >= 0 && act < R.a;
         if (MASK == SB_MASK_NONE) {
             const LaneSum z = pass_all<T, W, true, false>(x, Bits{}, R.a, c, part);
-            if (TOP)
-                top_of_all<T, W>(top, z.m, x, R.a, part, reinterpret_cast<uint64_t*>(sh) + warp * CANDIDATES,
-                                 &counts[warp]);
-            s = whole_all<T, W, true>(z, x, R.a, c, part, sums);
+            if (TOP) {
+                top_x[warp][lane] = sorted_down<2>(z.m);
+                if (tid == 0) counts[warp] = 0;
+                if (W == 1) __syncwarp();
+            }
+            s = whole_all<T, W, true>(z, x, R.a, c, part, sums);  // synchronises four warps
+            if (TOP) {
+                int* count = &counts[W == 1 ? warp : 0];
+                uint64_t* cand = reinterpret_cast<uint64_t*>(sh) + (W == 1 ? warp * CANDIDATES : 0);
+                // -inf is never listed
+                const float low = fmaxf(kth_peak<W>(top_x + (W == 1 ? warp : 0), o.top), -3.4028235e38f);
+                if (z.m >= low) list_from<T, W>(low, x, R.a, part, cand, W * CANDIDATES, count);
+                if (W == 1) __syncwarp();
+                else __syncthreads();
+                joined = *count <= W * CANDIDATES;
+                if (!joined) top_of_part<T, W>(top, x, R.a, part);
+                else if (part == 0) top_of_list(top, cand, *count);
+            }
         } else {
-            const Bits bits = stage<MASK, 32 * W>(sh_bits, R, row, W == 1 ? lane : threadIdx.x);
+            const Bits bits = stage<MASK, 32 * W>(sh_bits, R, row, tid);
             if (W == 1) __syncwarp();
             else __syncthreads();
             legal = legal && bits.test((int)act);
             pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, part);
         }
-        if (TOP && W > 1) {
+        if (TOP && W > 1 && !joined) {
             top_x[warp][lane] = top.x;
             top_a[warp][lane] = top.a;
         }
         if (MASK != SB_MASK_NONE) s = whole<W>(s, c, sums);
-        else if (TOP && W > 1) __syncthreads();
+        else if (TOP && W > 1 && !joined) __syncthreads();
         const float2 st = stats_of(s);
         if (W == 1 || warp == 0) {
             if (lane == 0) {
@@ -61,7 +76,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
                 if (o.row_stats) *reinterpret_cast<float2*>(o.row_stats + 2 * row) = st;
             }
             if (TOP) {
-                if (W > 1)
+                if (W > 1 && !joined)
                     for (int w = 1; w < W; ++w) top.offer(lane < o.top ? top_x[w][lane] : NEG_INF, top_a[w][lane]);
                 if (lane < o.top) {
                     const bool some = top.x > NEG_INF;

@@ -592,56 +592,80 @@ __device__ __forceinline__ Sum whole_all(LaneSum z, const T* x, int a, float c, 
     return r;
 }
 
-// A warp's k best of its part of an unmasked row.  The k-th largest of the
-// lanes' largest logits bounds the k-th best from below, so only the lanes that
-// reach it look through their elements again (from cache), and of those only
-// what reaches it is put in order.
-constexpr int CANDIDATES = 512;
-template <typename T, int W>
-__device__ __forceinline__ void top_of_all(Top& top, float mine, const T* x, int a, int part, uint64_t* cand, int* count) {
+// The k best of an unmasked row.  The k-th largest of the lanes' largest logits
+// bounds the k-th best from below, so only the lanes that reach it look through
+// their elements again (from cache), and of those only what reaches it is
+// listed: k elements and a few more, in any order, which one warp then sorts.
+constexpr int CANDIDATES = 512;  // for each of the row's warps
+
+// The warp's values in descending order, lane by lane, from d0 = 1 unsorted or
+// from d0 = 16 where the first half rises and the second falls.
+template <int N0> __device__ __forceinline__ float sorted_down(float v) {
     const int lane = threadIdx.x & 31;
-    Top bar = top;
-    bar.fill(mine, lane);
-    const float low = fmaxf(bar.bar_x, -3.4028235e38f);  // -inf is never listed
-    if (lane == 0) *count = 0;
-    __syncwarp();
+#pragma unroll
+    for (int n = N0; n <= 32; n <<= 1) {
+#pragma unroll
+        for (int d = n >> 1; d; d >>= 1) {
+            const float o = __shfl_xor_sync(ALL, v, d);
+            v = ((lane & d) == 0) == ((lane & n) == 0) ? fmaxf(v, o) : fminf(v, o);
+        }
+    }
+    return v;
+}
+
+// `peaks`: every warp's lanes' largest logits, sorted; returns the k-th of all.
+template <int W> __device__ __forceinline__ float kth_peak(const float (*peaks)[32], int k) {
+    const int lane = threadIdx.x & 31;
+    float v = peaks[0][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v = sorted_down<32>(fmaxf(v, peaks[w][31 - lane]));
+    return __shfl_sync(ALL, v, k - 1);
+}
+
+// This lane's elements of `low` and more, into cand[0 .. limit).
+template <typename T, int W>
+__device__ __forceinline__ void list_from(float low, const T* x, int a, int part, uint64_t* cand, int limit, int* count) {
+    constexpr int E = Chunk<T>::E;
     const Deal<T, W> deal(x, a, part);
     auto keep = [&](int b) {
         const int at = atomicAdd(count, 1);
-        if (at < CANDIDATES) cand[at] = (uint64_t)b << 32 | __float_as_uint(to_f(x[b]));
+        if (at < limit) cand[at] = (uint64_t)b << 32 | __float_as_uint(to_f(x[b]));
     };
-    if (mine >= low) {
-        constexpr int E = Chunk<T>::E;
-        for (int i = deal.first; i < deal.chunks; i += 32 * W) {
-            Chunk<T> q;
-            q.load(x + deal.head + i * E);
-            if (q.max() >= low) {
-                uint32_t hit = 0;
+    for (int i = deal.first; i < deal.chunks; i += 32 * W) {
+        Chunk<T> q;
+        q.load(x + deal.head + i * E);
+        if (q.max() >= low) {
+            uint32_t hit = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) hit |= q.get(e) >= low ? 1u << e : 0u;
-                for (; hit; hit &= hit - 1) keep(deal.head + i * E + __ffs(hit) - 1);
-            }
-        }
-        if (deal.end < a && to_f(x[deal.end]) >= low) keep(deal.end);
-    }
-    __syncwarp();
-    const int n = *count;
-    if (n <= CANDIDATES) {
-        for (int i = 0; i < n; i += 32) {
-            const uint64_t q = i + lane < n ? cand[i + lane] : 0;
-            const float v = i + lane < n ? __uint_as_float((uint32_t)q) : NEG_INF;
-            if (i == 0) top.fill(v, (int)(q >> 32));
-            else top.offer(v, (int)(q >> 32));
-        }
-    } else {  // a row of equal or sorted logits: every lane's elements in turn
-        const int rounds = (deal.chunks + 32 * W - 1) / (32 * W) * Chunk<T>::E;
-        top.offer(deal.end < a ? to_f(x[deal.end]) : NEG_INF, deal.end);
-        for (int i = 0; i < rounds; ++i) {
-            const int ch = deal.first + i / Chunk<T>::E * 32 * W, b = deal.head + ch * Chunk<T>::E + i % Chunk<T>::E;
-            top.offer(ch < deal.chunks ? to_f(x[b]) : NEG_INF, b);
+            for (int e = 0; e < E; ++e) hit |= q.get(e) >= low ? 1u << e : 0u;
+            for (; hit; hit &= hit - 1) keep(deal.head + i * E + __ffs(hit) - 1);
         }
     }
-    __syncwarp();
+    if (deal.end < a && to_f(x[deal.end]) >= low) keep(deal.end);
+}
+
+__device__ __forceinline__ void top_of_list(Top& top, const uint64_t* cand, int n) {
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < n; i += 32) {
+        const uint64_t q = i + lane < n ? cand[i + lane] : 0;
+        const float v = i + lane < n ? __uint_as_float((uint32_t)q) : NEG_INF;
+        if (i == 0) top.fill(v, (int)(q >> 32));
+        else top.offer(v, (int)(q >> 32));
+    }
+}
+
+// Where too many reach the bound (equal or sorted logits): a warp's part, all
+// lanes' elements in turn.
+template <typename T, int W>
+__device__ __forceinline__ void top_of_part(Top& top, const T* x, int a, int part) {
+    constexpr int E = Chunk<T>::E;
+    const Deal<T, W> deal(x, a, part);
+    const int rounds = (deal.chunks + 32 * W - 1) / (32 * W) * E;
+    top.offer(deal.end < a ? to_f(x[deal.end]) : NEG_INF, deal.end);
+    for (int i = 0; i < rounds; ++i) {
+        const int ch = deal.first + i / E * 32 * W, b = deal.head + ch * E + i % E;
+        top.offer(ch < deal.chunks ? to_f(x[b]) : NEG_INF, b);
+    }
 }
 
 // ---- gradient rows ---------------------------------------------------------------------

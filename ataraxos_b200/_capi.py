@@ -16,6 +16,8 @@ _LIB_DIR = Path(__file__).resolve().parent / "_lib"
 # reading or writing out of range; it is slower and meant for loaded records.
 DEBUG = os.environ.get("ATARAXOS_B200_DEBUG", "0") not in ("", "0")
 LIB_PATH = _LIB_DIR / ("libstratego_b200_debug.so" if DEBUG else "libstratego_b200.so")
+# the torch operators of ataraxos_b200.policy over either library
+TORCH_LIB_PATH = _LIB_DIR / "libstratego_b200_torch.so"
 
 SB_OK, SB_E_ARG, SB_E_CUDA, SB_E_NOPOOL = 0, -1, -2, -3
 SB_DTYPE_F32, SB_DTYPE_BF16, SB_DTYPE_F16 = 0, 1, 2

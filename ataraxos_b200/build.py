@@ -25,6 +25,10 @@ DEBUG_LIB_PATH = LIB_DIR / "libstratego_b200_debug.so"
 SOURCES = [CSRC / f for f in ("sb_kernels.cu", "sb_logprobs.cu", "sb_distill.cu", "sb_policy_small.cu")]
 DEPS = SOURCES + [CSRC / "sb_device.cuh", CSRC / "sb_error.h", CSRC / "sb_policy.cuh", INCLUDE / "stratego_b200.h"]
 
+# the policy operators as torch operators: C++ against torch's headers, no CUDA code
+TORCH_LIB_PATH = LIB_DIR / "libstratego_b200_torch.so"
+TORCH_SOURCE = CSRC / "sb_torch.cpp"
+
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
@@ -39,11 +43,11 @@ def nvcc() -> str:
     raise FileNotFoundError("nvcc not found: the CUDA toolkit is needed to build libstratego_b200.so")
 
 
-def up_to_date(path: Path = LIB_PATH) -> bool:
+def up_to_date(path: Path = LIB_PATH, deps: list[Path] | None = None) -> bool:
     if not path.exists():
         return False
     t = path.stat().st_mtime
-    return all(d.stat().st_mtime <= t for d in DEPS)
+    return all(d.stat().st_mtime <= t for d in (DEPS if deps is None else deps))
 
 
 def _compile(path: Path, extra: list[str], verbose: bool) -> None:
@@ -64,12 +68,31 @@ def _compile(path: Path, extra: list[str], verbose: bool) -> None:
         os.replace(lib, path)
 
 
+def _compile_torch(verbose: bool) -> None:
+    import torch
+
+    LIB_DIR.mkdir(exist_ok=True)
+    root = Path(torch.__file__).resolve().parent
+    tmp = LIB_DIR / f".{TORCH_LIB_PATH.name}.{os.getpid()}.tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           "-isystem", str(root / "include"), "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(Path(nvcc()).resolve().parent.parent / "include"), str(TORCH_SOURCE), f"-L{root / 'lib'}",
+           "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, TORCH_LIB_PATH)
+
+
 def build(force: bool = False, verbose: bool = False, debug: bool = True) -> Path:
-    """Build the production library (and, with ``debug``, the bounds-checking one)."""
+    """Build the production library (with ``debug``, the bounds-checking one too) and the torch operators over it."""
     if force or not up_to_date(LIB_PATH):
         _compile(LIB_PATH, [], verbose)
     if debug and (force or not up_to_date(DEBUG_LIB_PATH)):
         _compile(DEBUG_LIB_PATH, ["-DSB_DEBUG_BOUNDS"], verbose)
+    if force or not up_to_date(TORCH_LIB_PATH, [TORCH_SOURCE, INCLUDE / "stratego_b200.h"]):
+        _compile_torch(verbose)
     return LIB_PATH
 
 

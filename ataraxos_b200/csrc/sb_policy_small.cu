@@ -7,14 +7,15 @@
 // turn.  Loads are one element wide, so rows may lie at any stride or
 // offset; the lanes of a row read neighbouring elements.  A gradient is put
 // together in shared memory and stored as the contiguous block that four rows
-// are.
+// are.  The kernels are bound by their instructions (about 100 a row and
+// direction), so the actions of a lane are a constant, and by latency: the CTAs
+// per SM of their launch bounds were the fastest of 6 to 12.
 #include "sb_policy.cuh"
 
 namespace sb {
 namespace {
 
 constexpr int G = 8;             // lanes of a row
-constexpr int NI = SMALL / G;    // actions of a lane
 constexpr int RW = 32 / G;       // rows of a warp
 
 __device__ __forceinline__ float group_max(float v) {
@@ -29,15 +30,15 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 // One lane's actions of a row: their logits (-inf where not legal) and bit i
-// for a legal l + 8 i.
-struct Part {
+// for a legal l + 8 i.  NI: actions of a lane, at least ceil(A / 8).
+template <int NI> struct Part {
     float v[NI];
     uint32_t ok;
 };
 
-template <typename T>
-__device__ __forceinline__ Part load_part(const Rows& R, int kind, int64_t row, bool live, int l) {
-    Part p;
+template <typename T, int NI>
+__device__ __forceinline__ Part<NI> load_part(const Rows& R, int kind, int64_t row, bool live, int l) {
+    Part<NI> p;
     p.ok = 0;
     const T* x = static_cast<const T*>(R.x) + row * R.stride + l;
     const uint8_t* m = R.mask + row * R.mask_stride;
@@ -58,26 +59,37 @@ __device__ __forceinline__ Part load_part(const Rows& R, int kind, int64_t row, 
     return p;
 }
 
-// The row's sum, in all of its lanes, over the lane's actions in `ok`.
-template <bool ENT>
-__device__ __forceinline__ Sum sum_part(const Part& p, uint32_t ok, float c) {
+// The row's sum, in all of its lanes, over the lane's actions in `ok` (ALL: of
+// all, as the others are -inf already).  The maximum's own 1 is taken off the
+// lanes' sums at the end, or left out of them one by one where it is nearly
+// all of the mass.
+template <bool ENT, int NI>
+__device__ __forceinline__ Sum sum_part(const Part<NI>& p, uint32_t ok, float c) {
+    auto at = [&](int i) { return ok == ALL || (ok >> i) & 1 ? p.v[i] : NEG_INF; };
     Sum s = no_sum();
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-        if ((ok >> i) & 1) s.m = fmaxf(s.m, p.v[i]);
-    s.m = group_max(s.m);
+    for (int i = 0; i < NI; ++i) s.m = fmaxf(s.m, at(i));
+    const float mine = s.m;
+    s.m = group_max(mine);
     const float ref = s.m == NEG_INF ? 0.f : s.m;
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-        if ((ok >> i) & 1) {
-            const float d = (p.v[i] - ref) * c, e = exp2_(d);
-            if (p.v[i] == ref) s.n += 1.f;
-            else s.r += e;
-            if (ENT) s.t = fmaf(e, fmaxf(d, -1e4f), s.t);
-        }
-    s.n = group_sum(s.n);
-    s.r = group_sum(s.r);
+    for (int i = 0; i < NI; ++i) {
+        const float d = (at(i) - ref) * c, e = exp2_(d);
+        s.r += e;
+        if (ENT) s.t = fmaf(e, fmaxf(d, -1e4f), s.t);
+    }
+    const bool top = mine == s.m && s.m > NEG_INF;
+    const float all = s.r;
+    s.n = group_sum(top ? 1.f : 0.f);
+    s.r = group_sum(top ? all - 1.f : all);
     if (ENT) s.t = group_sum(s.t);
+    if (__any_sync(ALL, s.n == 1.f && s.r < 0.015625f)) {
+        float rest = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) rest += at(i) == ref ? 0.f : exp2_((at(i) - ref) * c);
+        rest = group_sum(rest);
+        if (s.n == 1.f && s.r < 0.015625f) s.r = rest;
+    }
     return s;
 }
 
@@ -88,8 +100,8 @@ __device__ __forceinline__ bool legal_in(uint32_t ok, int64_t a, int actions) {
     return ((__shfl_sync(ALL, ok, b % G, G) >> (b / G)) & 1) && in;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) small_logprobs_kernel(Rows R, int kind, sb_logprobs o) {
+template <typename T, int NI>
+__global__ void __launch_bounds__(WARPS * 32, 10) small_logprobs_kernel(Rows R, int kind, sb_logprobs o) {
     const int lane = threadIdx.x & 31, l = lane % G;
     const float c = R.inv_t * LOG2E;
     const int64_t step = (int64_t)gridDim.x * (WARPS * RW);
@@ -100,9 +112,9 @@ __global__ void __launch_bounds__(WARPS * 32) small_logprobs_kernel(Rows R, int 
         if (live && o.actions) act = load_index(o.actions, o.action_bytes, row);
         const bool in = act >= 0 && act < R.a;
         const float xa = in ? to_f(static_cast<const T*>(R.x)[row * R.stride + act]) : 0.f;
-        const Part p = load_part<T>(R, kind, row, live, l);
+        const Part<NI> p = load_part<T, NI>(R, kind, row, live, l);
         const bool legal = legal_in(p.ok, act, R.a);
-        const Sum s = sum_part<true>(p, p.ok, c);
+        const Sum s = sum_part<true>(p, ALL, c);
         const float2 st = stats_of(s);
         if (live && l == 0) {
             if (o.logprob) o.logprob[row] = act == -1 ? 0.f : legal ? (xa - st.x) * R.inv_t - st.y : NEG_INF;
@@ -154,8 +166,8 @@ __device__ __forceinline__ void store_rows(const T* sh, T* out, int a, int64_t r
     __syncwarp();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) small_logprobs_backward_kernel(Rows R, int kind, sb_logprobs f,
+template <typename T, int NI>
+__global__ void __launch_bounds__(WARPS * 32, 8) small_logprobs_backward_kernel(Rows R, int kind, sb_logprobs f,
                                                                              sb_logprobs_grad g) {
     __shared__ __align__(16) T rows[WARPS][RW * SMALL];
     __shared__ float adds[WARPS][RW][SMALL];
@@ -178,24 +190,25 @@ __global__ void __launch_bounds__(WARPS * 32) small_logprobs_backward_kernel(Row
             st = *reinterpret_cast<const float2*>(f.row_stats + 2 * row);
             h = f.entropy[row];
         }
-        const Part p = load_part<T>(R, kind, row, live, l);
+        const Part<NI> p = load_part<T, NI>(R, kind, row, live, l);
         if (!legal_in(p.ok, act, R.a)) {
             act = -1;
             ga = 0.f;
         }
+        const int mine = act >= 0 && (int)act % G == l ? (int)act / G : -1;  // the given action, if it is the lane's
         float total = ga;
         if (g.g_top) {  // the alternatives are all different actions
             for (int i = l; i < R.a; i += G) add[i] = 0.f;
             __syncwarp();
-            float mine = 0.f;
+            float shares = 0.f;
             for (int k = l; live && k < f.top; k += G) {
                 const int64_t a = f.top_action[row * f.top + k];
                 if (a >= 0) {
                     add[a] = g.g_top[row * f.top + k];
-                    mine += add[a];
+                    shares += add[a];
                 }
             }
-            total += group_sum(mine);
+            total += group_sum(shares);
             __syncwarp();
         }
         const RowGrad r = {st.x, st.y, -(total + gh * h), -gh, 0.f};
@@ -203,7 +216,7 @@ __global__ void __launch_bounds__(WARPS * 32) small_logprobs_backward_kernel(Row
         for (int i = 0; i < NI; ++i) {
             const int a = l + G * i;
             if (a < R.a) {
-                const float e = (act == a ? ga : 0.f) + (g.g_top ? add[a] : 0.f);
+                const float e = (i == mine ? ga : 0.f) + (g.g_top ? add[a] : 0.f);
                 sh[q * R.a + a] = from_f<T>((p.ok >> i) & 1 ? grad_of<true>(p.v[i], r, r.c0, e, R.inv_t) : 0.f);
             }
         }
@@ -223,8 +236,8 @@ __device__ __forceinline__ int small_teacher(const Rows& R, const sb_distill& d,
     return legal_in(ok, a, R.a) && !(*v == NEG_INF) ? (int)a : -1;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) small_distill_kernel(Rows R, int kind, sb_distill d) {
+template <typename T, int NI>
+__global__ void __launch_bounds__(WARPS * 32, 10) small_distill_kernel(Rows R, int kind, sb_distill d) {
     const int lane = threadIdx.x & 31, l = lane % G;
     const float c = R.inv_t * LOG2E, tc = d.tail ? 1.f : R.inv_t;
     const int64_t step = (int64_t)gridDim.x * (WARPS * RW);
@@ -232,8 +245,8 @@ __global__ void __launch_bounds__(WARPS * 32) small_distill_kernel(Rows R, int k
         const int64_t row = row0 + lane / G;
         const bool live = row < R.n;
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        const Part p = load_part<T>(R, kind, row, live, l);
-        const float2 st = stats_of(sum_part<false>(p, p.ok, c));
+        const Part<NI> p = load_part<T, NI>(R, kind, row, live, l);
+        const float2 st = stats_of(sum_part<false>(p, ALL, c));
         float2 tst = make_float2(0.f, 0.f);
         if (!d.tail) {
             float m = NEG_INF;
@@ -302,8 +315,8 @@ __global__ void __launch_bounds__(WARPS * 32) small_distill_kernel(Rows R, int k
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) small_distill_backward_kernel(Rows R, int kind, sb_distill d,
+template <typename T, int NI>
+__global__ void __launch_bounds__(WARPS * 32, 8) small_distill_backward_kernel(Rows R, int kind, sb_distill d,
                                                                             const float* g_loss, int64_t g_stride, T* grad) {
     __shared__ __align__(16) T rows[WARPS][RW * SMALL];
     __shared__ float weights[WARPS][RW][SMALL];
@@ -322,7 +335,7 @@ __global__ void __launch_bounds__(WARPS * 32) small_distill_backward_kernel(Rows
             st = s[0], co = s[1], te = s[2];
             w = g_loss[row * g_stride];
         }
-        const Part p = load_part<T>(R, kind, row, live, l);
+        const Part<NI> p = load_part<T, NI>(R, kind, row, live, l);
         for (int i = l; i < R.a; i += G) wt[i] = 0.f;
         uint32_t listed = 0;
         for (int k = l; k < (d.listed + G - 1) / G * G; k += G) {
@@ -360,44 +373,56 @@ Rows rows_of(const sb_logits* x) {
 
 unsigned small_grid(int64_t rows) { return grid_of(rows, 1) > 4 ? (grid_of(rows, 1) + RW - 1) / RW : 1; }
 
+// Call f(element type, actions of a lane) as constants.
 template <typename F>
 int by_type(const sb_logits* x, F f) {
-    if (x->dtype == SB_DTYPE_F32) return f((float*)nullptr);
-    if (x->dtype == SB_DTYPE_BF16) return f((__nv_bfloat16*)nullptr);
-    return f((__half*)nullptr);
+    auto sizes = [&](auto* t) {
+        const int n = (x->n_actions + G - 1) / G;
+        if (n <= 4) return f(t, std::integral_constant<int, 4>{});
+        if (n <= 8) return f(t, std::integral_constant<int, 8>{});
+        if (n <= 13) return f(t, std::integral_constant<int, 13>{});
+        return f(t, std::integral_constant<int, SMALL / G>{});
+    };
+    if (x->dtype == SB_DTYPE_F32) return sizes((float*)nullptr);
+    if (x->dtype == SB_DTYPE_BF16) return sizes((__nv_bfloat16*)nullptr);
+    return sizes((__half*)nullptr);
 }
 
 }  // namespace
 
 int small_logprobs(const sb_logits* x, const sb_logprobs& o, cudaStream_t st) {
-    return by_type(x, [&](auto* t) {
+    return by_type(x, [&](auto* t, auto ni) {
         using T = std::remove_pointer_t<decltype(t)>;
-        small_logprobs_kernel<T><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, o);
+        constexpr int NI = decltype(ni)::value;
+        small_logprobs_kernel<T, NI><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, o);
         return launched("small_logprobs_kernel launch");
     });
 }
 
 int small_logprobs_backward(const sb_logits* x, const sb_logprobs& f, const sb_logprobs_grad& g, cudaStream_t st) {
-    return by_type(x, [&](auto* t) {
+    return by_type(x, [&](auto* t, auto ni) {
         using T = std::remove_pointer_t<decltype(t)>;
-        small_logprobs_backward_kernel<T><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, f, g);
+        constexpr int NI = decltype(ni)::value;
+        small_logprobs_backward_kernel<T, NI><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, f, g);
         return launched("small_logprobs_backward_kernel launch");
     });
 }
 
 int small_distill(const sb_logits* x, const sb_distill& d, cudaStream_t st) {
-    return by_type(x, [&](auto* t) {
+    return by_type(x, [&](auto* t, auto ni) {
         using T = std::remove_pointer_t<decltype(t)>;
-        small_distill_kernel<T><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, d);
+        constexpr int NI = decltype(ni)::value;
+        small_distill_kernel<T, NI><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, d);
         return launched("small_distill_kernel launch");
     });
 }
 
 int small_distill_backward(const sb_logits* x, const sb_distill& d, const float* g_loss, int64_t g_stride, void* grad,
                            cudaStream_t st) {
-    return by_type(x, [&](auto* t) {
+    return by_type(x, [&](auto* t, auto ni) {
         using T = std::remove_pointer_t<decltype(t)>;
-        small_distill_backward_kernel<T><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, d, g_loss,
+        constexpr int NI = decltype(ni)::value;
+        small_distill_backward_kernel<T, NI><<<small_grid(x->n_rows), WARPS * 32, 0, st>>>(rows_of(x), x->mask_kind, d, g_loss,
                                                                                       g_stride, static_cast<T*>(grad));
         return launched("small_distill_backward_kernel launch");
     });

@@ -11,28 +11,29 @@ namespace {
 // teacher's own (maximum, log sum).
 
 // This lane's teacher entry of a round of 32: its action (-1 where it is left
-// out), logit and student logit.  Loaded before the mask is known (`load`),
-// so the three loads' latency passes beside the mask's, then checked.
+// out), logit and student logit.  The first round is loaded beside the mask
+// and looked at when that has come: a warp that waits for an action issues no
+// other load.
 struct Entry {
     int a;
     float v, x;
 };
-template <typename T>
-__device__ __forceinline__ Entry load_entry(const Rows& R, const sb_distill& d, const T* x, int64_t row, int k) {
-    Entry e = {-1, 0.f, 0.f};
-    if (k < d.listed) {
-        const int64_t a = load_index(d.teacher_actions, d.action_bytes, row * d.listed + k);
-        e.v = load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k);
-        if (a >= 0 && a < R.a && !(e.v == NEG_INF)) {
-            e.a = (int)a;
-            e.x = to_f(x[a]);
-        }
-    }
-    return e;
+struct Raw {
+    int64_t a;
+    float v;
+};
+__device__ __forceinline__ Raw load_raw(const sb_distill& d, int64_t row, int k) {
+    if (k >= d.listed) return {-1, NEG_INF};
+    return {load_index(d.teacher_actions, d.action_bytes, row * d.listed + k),
+            load_value(d.teacher_logits, d.teacher_dtype, row * d.listed + k)};
 }
-template <int MASK>
-__device__ __forceinline__ Entry check_entry(Entry e, Bits bits) {
-    if (MASK != SB_MASK_NONE && e.a >= 0 && !bits.test(e.a)) e.a = -1;
+template <typename T, int MASK>
+__device__ __forceinline__ Entry entry_of(const Rows& R, const T* x, Bits bits, Raw q) {
+    Entry e = {-1, q.v, 0.f};
+    if (q.a >= 0 && q.a < R.a && !(q.v == NEG_INF) && (MASK == SB_MASK_NONE || bits.test((int)q.a))) {
+        e.a = (int)q.a;
+        e.x = to_f(x[q.a]);
+    }
     return e;
 }
 
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        Entry e0 = load_entry(R, d, x, row, lane);
+        const Raw raw = load_raw(d, row, lane);
         Bits bits = {nullptr, 0};
         if (MASK != SB_MASK_NONE) bits = stage<MASK, 32 * W>(sh_bits, R, row, tid);
         // which actions are listed, as bits: needed at once to find an entry's
@@ -70,8 +71,8 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
         if (W == 1) __syncwarp();
         else __syncthreads();
         const Bits skip = {sh_skip, bits.p};
-        e0 = check_entry<MASK>(e0, bits);
-        auto entry = [&](int k0) { return k0 ? check_entry<MASK>(load_entry(R, d, x, row, k0 + lane), bits) : e0; };
+        const Entry e0 = entry_of<T, MASK>(R, x, bits, raw);
+        auto entry = [&](int k0) { return k0 ? entry_of<T, MASK>(R, x, bits, load_raw(d, row, k0 + lane)) : e0; };
         Sum s = no_sum();
         Top none;
         int legal = 0;
@@ -204,18 +205,19 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
         const float2* s = reinterpret_cast<const float2*>(d.row_stats + 6 * row);
         const float2 st = s[0], co = s[1], te = s[2];
         const float w = g_loss[row * g_stride];
-        Entry e0 = load_entry(R, d, x, row, lane);
+        const Raw raw = load_raw(d, row, lane);
         Bits bits = {nullptr, 0};
         if (MASK != SB_MASK_NONE) {
             bits = stage<MASK, 32 * W>(sh_bits, R, row, W == 1 ? lane : threadIdx.x);
             if (W == 1) __syncwarp();
             else __syncthreads();
         }
-        e0 = check_entry<MASK>(e0, bits);
+        auto entry = [&](int k0) { return entry_of<T, MASK>(R, x, bits, load_raw(d, row, k0 + lane)); };
+        const Entry e0 = entry_of<T, MASK>(R, x, bits, raw);
         const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
         const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
         for (int k0 = 0; k0 < d.listed; k0 += 32) {
-            const Entry e = k0 ? check_entry<MASK>(load_entry(R, d, x, row, k0 + lane), bits) : e0;
+            const Entry e = k0 ? entry(k0) : e0;
             float q = e.a >= 0 ? expf((e.v - te.x) * tc - te.y) : 0.f;
             // An action that is listed again takes all of its entries' weights:
             // each of its lanes adds them in the entries' order and stores the
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
             if (d.listed > 32 || __any_sync(ALL, e.a >= 0 && (peers & (peers - 1)))) {
                 q = 0.f;
                 for (int j0 = 0; j0 < d.listed; j0 += 32) {
-                    const Entry f = j0 == k0 ? e : check_entry<MASK>(load_entry(R, d, x, row, j0 + lane), bits);
+                    const Entry f = j0 == k0 ? e : entry(j0);
                     const float qf = f.a >= 0 ? expf((f.v - te.x) * tc - te.y) : 0.f;
                     for (int j = 0; j < 32 && j0 + j < d.listed; ++j) {
                         const int b = __shfl_sync(ALL, f.a, j);

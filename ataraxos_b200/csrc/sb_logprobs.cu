@@ -24,18 +24,18 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
     const int64_t step = (int64_t)gridDim.x * (WARPS / W);
     for (int64_t row = (int64_t)blockIdx.x * (WARPS / W) + (W == 1 ? warp : 0); row < R.n; row += step) {
         const T* x = static_cast<const T*>(R.x) + row * R.stride;
-        int64_t act = -1;
+        // the action's logit is asked for only when its mask is on the way too:
+        // a warp that waits for the action issues no other load
+        const int64_t act = o.actions ? load_index(o.actions, o.action_bytes, row) : -1;
         float xa = 0.f;
-        if (o.actions) {
-            act = load_index(o.actions, o.action_bytes, row);
-            if (act >= 0 && act < R.a) xa = to_f(x[act]);
-        }
         Sum s = no_sum();
         Top top;
         top.init(TOP ? o.top : 1);
         bool joined = false;  // the first warp's list is the row's
-        bool legal = act >= 0 && act < R.a;
+        bool legal;
         if (MASK == SB_MASK_NONE) {
+            legal = act >= 0 && act < R.a;
+            if (legal) xa = to_f(x[act]);
             const LaneSum z = pass_all<T, W, true, false>(x, Bits{}, R.a, c, part);
             if (TOP) {
                 top_x[warp][lane] = sorted_down<2>(z.m);
@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
             const Bits bits = stage<MASK, 32 * W>(sh_bits, R, row, tid);
             if (W == 1) __syncwarp();
             else __syncthreads();
-            legal = legal && bits.test((int)act);
+            legal = act >= 0 && act < R.a && bits.test((int)act);
+            if (legal) xa = to_f(x[act]);
             pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, part);
         }
         if (TOP && W > 1 && !joined) {
@@ -117,8 +118,6 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
             act = load_index(f.actions, f.action_bytes, row);
             ga = g.g_logprob[row * g.g_logprob_stride];
         }
-        const float xm = mine >= 0 ? to_f(x[mine]) : 0.f;
-        const float xa = act >= 0 && act < R.a ? to_f(x[act]) : 0.f;
         const float gh = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] : 0.f;
         const float2 st = *reinterpret_cast<const float2*>(f.row_stats + 2 * row);
         const float h = f.entropy[row];
@@ -130,6 +129,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
         }
         bool legal = act >= 0 && act < R.a;
         if (MASK != SB_MASK_NONE) legal = legal && bits.test((int)act);
+        const float xm = mine >= 0 ? to_f(x[mine]) : 0.f, xa = legal ? to_f(x[act]) : 0.f;
         const float total = warp_sum(add) + (legal ? ga : 0.f);
         const RowGrad r = {st.x, st.y, -(total + gh * h), -gh, -(total + gh * h)};
         const int2 own = grad_row<T, MASK, W, true>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);

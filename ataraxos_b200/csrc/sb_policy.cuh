@@ -685,17 +685,15 @@ __device__ __forceinline__ float grad_of(float x, const RowGrad& g, float c0, fl
 
 // One lane's chunk of a gradient row: the elements that are set in `field`,
 // the others 0.  Few are set: a loop over them, with the lane's slots in
-// shared memory to index by.
+// shared memory to index by.  `q`: the chunk's logits where they were loaded
+// whole (`wide`).
 template <typename T, bool ENT>
-__device__ __forceinline__ void grad_sparse(const T* x, T* g, int first, int a, uint32_t field, const RowGrad& r,
-                                            float inv_t, T* xs, T* gs) {
+__device__ __forceinline__ void grad_sparse(const T* x, T* g, int first, int a, uint32_t field, bool wide, Chunk<T> q,
+                                            const RowGrad& r, float inv_t, T* xs, T* gs) {
     constexpr int E = Chunk<T>::E;
-    const bool full = first >= 0 && first + E <= a, wide = full && ((intptr_t)(x + first) & 31) == 0;
     uint4* x4 = reinterpret_cast<uint4*>(xs);
     uint4* g4 = reinterpret_cast<uint4*>(gs);
-    Chunk<T> q;
     if (wide) {
-        q.load(x + first);
         x4[0] = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
         x4[1] = make_uint4(q.w[4], q.w[5], q.w[6], q.w[7]);
     }
@@ -706,7 +704,7 @@ __device__ __forceinline__ void grad_sparse(const T* x, T* g, int first, int a, 
         gs[e] = from_f<T>(grad_of<ENT>(to_f(wide ? xs[e] : x[first + e]), r, r.c0, 0.f, inv_t));
     }
     asm volatile("" ::: "memory");
-    if (full) {
+    if (first >= 0 && first + E <= a) {
         const uint4 u = g4[0], v = g4[1];
         q.w[0] = u.x, q.w[1] = u.y, q.w[2] = u.z, q.w[3] = u.w;
         q.w[4] = v.x, q.w[5] = v.y, q.w[6] = v.z, q.w[7] = v.w;
@@ -761,24 +759,35 @@ __device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, con
         T* gs = reinterpret_cast<T*>(sh + 4 * CHUNKS + (32 + lane) * SLOT);
         Chunk<T> zero;
         zero.fill(0);
-        int count = 0;
+        auto open = [&](int ch, uint32_t f) { return f != 0 || ch * E - e0 < 0 || ch * E - e0 + E > a; };
+        int count = 0, from = lo;  // listed chunks; the first one whose zeros are not stored
+#pragma unroll 2
         for (int c0 = lo; c0 < hi; c0 += 32) {
-            const int ch = c0 + lane, first = ch * E - e0;
-            const uint32_t f = ch < hi ? bits.field(first, E) : 0u;
-            const bool full = first >= 0 && first + E <= a;
-            const bool put = ch < hi && (f != 0 || !full);
+            const int ch = c0 + lane, to = min(c0 + 32, hi);
+            const uint32_t f = ch < hi ? bits.field(ch * E - e0, E) : 0u;
+            const bool put = ch < hi && open(ch, f);
             const unsigned b = __ballot_sync(ALL, put);
             if (put) list[count + __popc(b & ((1u << lane) - 1u))] = (uint32_t)ch | f << 16;
-            else if (ch < hi) zero.store(g + first);
             count += __popc(b);
-            if (count > CHUNKS - 32 || c0 + 32 >= hi) {
+            if (count > CHUNKS - 32 || to == hi) {
                 __syncwarp();
-                for (int i = lane; i < count; i += 32) {
+                // the first 32 listed chunks' logits come while the zeros go
+                const uint32_t v0 = lane < count ? list[lane] : 0u;
+                const int first0 = (int)(v0 & 0xffffu) * E - e0;
+                const bool wide = lane < count && first0 >= 0 && first0 + E <= a && ((intptr_t)(x + first0) & 31) == 0;
+                Chunk<T> q;
+                if (wide) q.load(x + first0);
+#pragma unroll 2
+                for (int k = from + lane; k < to; k += 32)
+                    if (!open(k, bits.field(k * E - e0, E))) zero.store(g + k * E - e0);
+                if (lane < count) grad_sparse<T, ENT>(x, g, first0, a, v0 >> 16, wide, q, r, inv_t, xs, gs);
+                for (int i = lane + 32; i < count; i += 32) {
                     const uint32_t v = list[i];
-                    grad_sparse<T, ENT>(x, g, (int)(v & 0xffffu) * E - e0, a, v >> 16, r, inv_t, xs, gs);
+                    grad_sparse<T, ENT>(x, g, (int)(v & 0xffffu) * E - e0, a, v >> 16, false, q, r, inv_t, xs, gs);
                 }
                 __syncwarp();
                 count = 0;
+                from = to;
             }
         }
     }
@@ -840,14 +849,22 @@ int dispatch(const sb_logits* x, bool wide, F f) {
 inline int64_t row_bytes(const sb_logits* x) { return (int64_t)x->n_actions * (x->dtype == SB_DTYPE_F32 ? 4 : 2); }
 
 // Four warps per row where one would have a long chain of loads for it: more
-// than 4 KB of an unmasked row (32 elements a lane and turn), a mask of more
-// than 16,384 actions (2 KB of staged bits a warp), or a masked gradient row
-// of more than 64 KB (1 KB of zeros a turn).  Splitting a shorter masked row
-// costs more than it gives: each warp pays for its own joins.
+// than 4 KB of an unmasked row (32 elements a lane and turn) or a mask of more
+// than 16,384 actions (2 KB of staged bits a warp).  Splitting a shorter masked
+// row costs more than it gives: each warp pays for its own joins.
 inline bool wide_forward(const sb_logits* x) {
     return x->mask_kind == SB_MASK_NONE ? row_bytes(x) > 4096 : x->n_actions > 16384;
 }
-inline bool wide_backward(const sb_logits* x) { return row_bytes(x) > (x->mask_kind == SB_MASK_NONE ? 4096 : 65536); }
+// A gradient's elements do not depend on who computes them, so here the rows
+// count too: four warps a masked row while there are fewer than 8 rows an SM
+// (64 rows of 10,000 f32: 4.2 against 9.2 us; 4096 rows: 26.5 against 21.4), and
+// above 64 KB a row (1 KB of zeros a turn).
+inline bool wide_backward(const sb_logits* x) {
+    if (x->mask_kind == SB_MASK_NONE) return row_bytes(x) > 4096;
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || sm_count(dev, &sms) != SB_OK) return false;
+    return row_bytes(x) > 65536 || (row_bytes(x) > 4096 && x->n_rows < 8 * (int64_t)sms);
+}
 
 // Rows of up to SMALL actions: sb_policy_small.cu.
 }  // namespace

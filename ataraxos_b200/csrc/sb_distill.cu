@@ -76,17 +76,32 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
         Sum s = no_sum();
         Top none;
         int legal = 0;
-        if (MASK == SB_MASK_NONE)
-            s = whole_all<T, W, false>(pass_all<T, W, false, false>(x, skip, R.a, c, part), x, R.a, c, part, sums);
-        else legal = pass_masked<T, W, false, false, false>(s, none, x, bits, bits, R.a, c, list, part);
-        if (W > 1 && MASK != SB_MASK_NONE && lane == 0) counts[warp] = legal;
-        if (MASK != SB_MASK_NONE) s = whole<W>(s, c, sums);
-        if (W > 1 && MASK != SB_MASK_NONE) {
-            legal = 0;
+        bool dense = MASK == SB_MASK_NONE;
+        auto read_whole = [&](auto f) {
+            constexpr int F = decltype(f)::kind;
+            return whole_all<T, W, false, F>(pass_all<T, W, false, F>(x, f, R.a, c, part), x, f, R.a, c, part, sums);
+        };
+        if (MASK == SB_MASK_NONE) {
+            s = read_whole(Filter<0>{});
+            legal = R.a;
+        } else {
+            legal = pass_masked<T, W, false, false, false>(s, none, x, bits, bits, R.a, c, list, part);
+            if (W > 1) {
+                if (lane == 0) counts[warp] = legal;
+                s = whole<W>(s, c, sums);
+                legal = 0;
 #pragma unroll
-            for (int w = 0; w < W; ++w) legal += counts[w];
+                for (int w = 0; w < W; ++w) legal += counts[w];
+            } else if (legal < 0) {
+                dense = true;
+                s = read_whole(Filter<1>{bits, bits});
+                int mine = 0;
+                for (int i = lane; i < (R.a + 31) >> 5; i += 32) mine += __popc(bits.word(i));
+                legal = __reduce_add_sync(ALL, mine);
+            } else {
+                s = whole<W>(s, c, sums);
+            }
         }
-        if (MASK == SB_MASK_NONE) legal = R.a;
         const float2 st = stats_of(s);
         float loss = 0.f, total = 0.f, share = 0.f;
         float2 tst = make_float2(0.f, 0.f);
@@ -159,7 +174,9 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
                 }
                 Sum rest = no_sum();
                 if (MASK == SB_MASK_NONE) {
-                    rest = whole_all<T, W, false>(pass_all<T, W, false, true>(x, skip, R.a, c, part), x, R.a, c, part, sums);
+                    rest = read_whole(Filter<2>{skip, skip});
+                } else if (W == 1 && dense) {
+                    rest = read_whole(Filter<3>{bits, skip});
                 } else {
                     pass_masked<T, W, false, false, true>(rest, none, x, bits, skip, R.a, c, list, part);
                     rest = whole<W>(rest, c, sums);

@@ -8,7 +8,7 @@ namespace {
 // ---- forward: given actions, entropy, top alternatives -----------------------------
 
 template <typename T, int MASK, int W, bool TOP>
-__global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprobs o) {
+__device__ __forceinline__ void logprobs_rows(const Rows& R, const sb_logprobs& o) {
     extern __shared__ uint4 dyn[];
     __shared__ Sum sums[WARPS];
     __shared__ float top_x[WARPS][32];
@@ -32,42 +32,53 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
         Top top;
         top.init(TOP ? o.top : 1);
         bool joined = false;  // the first warp's list is the row's
-        bool legal;
-        if (MASK == SB_MASK_NONE) {
-            legal = act >= 0 && act < R.a;
-            if (legal) xa = to_f(x[act]);
-            const LaneSum z = pass_all<T, W, true, false>(x, Bits{}, R.a, c, part);
+        bool dense = MASK == SB_MASK_NONE;
+        // the whole row, with up to `limit` candidates for its k best
+        auto read_whole = [&](auto f, int limit) {
+            constexpr int F = decltype(f)::kind;
+            const LaneSum z = pass_all<T, W, true, F>(x, f, R.a, c, part);
             if (TOP) {
                 top_x[warp][lane] = sorted_down<2>(z.m);
                 if (tid == 0) counts[warp] = 0;
                 if (W == 1) __syncwarp();
             }
-            s = whole_all<T, W, true>(z, x, R.a, c, part, sums);  // synchronises four warps
+            const Sum r = whole_all<T, W, true, F>(z, x, f, R.a, c, part, sums);  // synchronises four warps
             if (TOP) {
                 int* count = &counts[W == 1 ? warp : 0];
-                uint64_t* cand = reinterpret_cast<uint64_t*>(sh) + (W == 1 ? warp * CANDIDATES : 0);
+                uint64_t* cand = reinterpret_cast<uint64_t*>(
+                    MASK == SB_MASK_NONE ? sh + (W == 1 ? warp * 8 * CANDIDATES : 0) : reinterpret_cast<uint8_t*>(list));
                 // -inf is never listed
                 const float low = fmaxf(kth_peak<W>(top_x + (W == 1 ? warp : 0), o.top), -3.4028235e38f);
-                if (z.m >= low) list_from<T, W>(low, x, R.a, part, cand, W * CANDIDATES, count);
+                if (z.m >= low) list_from<T, W, F>(low, x, f, R.a, part, cand, limit, count);
                 if (W == 1) __syncwarp();
                 else __syncthreads();
-                joined = *count <= W * CANDIDATES;
-                if (!joined) top_of_part<T, W>(top, x, R.a, part);
+                joined = *count <= limit;
+                if (!joined) top_of_part<T, W, F>(top, x, f, R.a, part);
                 else if (part == 0) top_of_list(top, cand, *count);
             }
+            return r;
+        };
+        bool legal;
+        if (MASK == SB_MASK_NONE) {
+            legal = act >= 0 && act < R.a;
+            if (legal) xa = to_f(x[act]);
+            s = read_whole(Filter<0>{}, W * CANDIDATES);
         } else {
             const Bits bits = stage<MASK, 32 * W>(sh_bits, R, row, tid);
             if (W == 1) __syncwarp();
             else __syncthreads();
             legal = act >= 0 && act < R.a && bits.test((int)act);
             if (legal) xa = to_f(x[act]);
-            pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, part);
+            const int taken = pass_masked<T, W, true, TOP, false>(s, top, x, bits, bits, R.a, c, list, part);
+            if constexpr (W == 1)
+                if (taken < 0) s = read_whole(Filter<1>{bits, bits}, PASS_BYTES / 8);
+            dense = W == 1 && taken < 0;
         }
         if (TOP && W > 1 && !joined) {
             top_x[warp][lane] = top.x;
             top_a[warp][lane] = top.a;
         }
-        if (MASK != SB_MASK_NONE) s = whole<W>(s, c, sums);
+        if (!dense) s = whole<W>(s, c, sums);
         else if (TOP && W > 1 && !joined) __syncthreads();
         const float2 st = stats_of(s);
         if (W == 1 || warp == 0) {
@@ -90,6 +101,21 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(Rows R, sb_logprob
         if (W > 1) __syncthreads();
         else __syncwarp();
     }
+}
+
+template <typename T, int MASK, int W, bool TOP>
+__global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(const __grid_constant__ Rows R,
+                                                             const __grid_constant__ sb_logprobs o) {
+    logprobs_rows<T, MASK, W, TOP>(R, o);
+}
+
+// Masked rows with alternatives, a warp each: held to 48 registers, for the
+// sort takes 72 otherwise and the loads' latency wants the warps (16,384 rows,
+// 20 alternatives: 34.8 -> 26.6 us).
+template <typename T, int MASK>
+__global__ void __launch_bounds__(WARPS * 32, 10) logprobs_top_kernel(const __grid_constant__ Rows R,
+                                                                     const __grid_constant__ sb_logprobs o) {
+    logprobs_rows<T, MASK, 1, true>(R, o);
 }
 
 template <typename T, int MASK, int W>
@@ -173,10 +199,11 @@ int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream)
         const int smem = M != SB_MASK_NONE ? WARPS / W * bits_bytes(R.a) + WARPS * PASS_BYTES
                          : out->top        ? WARPS * 8 * CANDIDATES
                                            : 0;
-        if (out->top)
-            logprobs_kernel<T, M, W, true><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
-        else
-            logprobs_kernel<T, M, W, false><<<grid_of(R.n, W), WARPS * 32, smem, (cudaStream_t)stream>>>(R, *out);
+        const auto st = (cudaStream_t)stream;
+        const unsigned grid = grid_of(R.n, W);
+        if (!out->top) logprobs_kernel<T, M, W, false><<<grid, WARPS * 32, smem, st>>>(R, *out);
+        else if constexpr (M != SB_MASK_NONE && W == 1) logprobs_top_kernel<T, M><<<grid, WARPS * 32, smem, st>>>(R, *out);
+        else logprobs_kernel<T, M, W, true><<<grid, WARPS * 32, smem, st>>>(R, *out);
         return launched("logprobs_kernel launch");
     });
 }

@@ -87,6 +87,34 @@ template <typename T> struct Chunk {
                      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                      : "l"(p));
     }
+    // The chunk at row[first], whatever its alignment: where it is not a sector
+    // of its own, from the 16-byte pieces that it touches, if those are the
+    // row's (false: load it element by element).
+    __device__ __forceinline__ bool load_near(const T* row, int first, int a) {
+        const intptr_t p = (intptr_t)(row + first);
+        if (first < 0 || first + E > a) return false;
+        if ((p & 31) == 0) {
+            load(row + first);
+            return true;
+        }
+        const int off = (int)(p & 15);
+        const intptr_t base = p - off;
+        if (base < (intptr_t)row || base + (off ? 48 : 32) > (intptr_t)(row + a)) return false;
+        const uint4* g = reinterpret_cast<const uint4*>(base);
+        const uint4 x = __ldg(g), y = __ldg(g + 1), z = off ? __ldg(g + 2) : make_uint4(0, 0, 0, 0);
+        uint32_t v[12] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+        if (off & 4) {
+#pragma unroll
+            for (int i = 0; i < 11; ++i) v[i] = v[i + 1];
+        }
+        if (off & 8) {
+#pragma unroll
+            for (int i = 0; i < 9; ++i) v[i] = v[i + 2];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * (off & 3));
+        return true;
+    }
     __device__ __forceinline__ void store(T* p) const {
         asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                      "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -414,7 +442,9 @@ struct Top {
 // actions come out in ascending order and are dealt to the lanes in turn, so
 // the sums' order, and with it every bit of the result, is the same for any
 // kind of mask and wherever its rows lie.  SKIP leaves out the actions of
-// `skip`.  Returns how many actions were taken.
+// `skip`.  Returns how many actions were taken, or -1, none taken, for a row of
+// one warp that is better read whole (pass_all): over half of its first words
+// hold a legal action, and over an eighth of their actions are legal.
 template <typename T, int W, bool ENT, bool TOP, bool SKIP>
 __device__ __forceinline__ int pass_masked(Sum& s, Top& top, const T* x, Bits bits, Bits skip, int a, float c,
                                            uint16_t* list, int part) {
@@ -436,6 +466,11 @@ __device__ __forceinline__ int pass_masked(Sum& s, Top& top, const T* x, Bits bi
             n += __popc(m);
         }
         __syncwarp();
+        if (W == 1 && !SKIP && w0 == 0 && 2 * n > min(words, WORDS)) {
+            int count = 0;
+            for (int j = lane; j < n; j += 32) count += __popc(word(some[j]));
+            if (__reduce_add_sync(ALL, count) > 4 * min(words, WORDS)) return -1;
+        }
         for (int j = 0; j < n; j += 32) {
             const int i = j + lane < n ? some[j + lane] : 0;
             uint32_t w = j + lane < n ? word(i) : 0u;
@@ -523,9 +558,22 @@ template <typename T, int W> struct Deal {
     }
 };
 
+// Which actions of a whole row count: with F & 1 only the legal ones, with
+// F & 2 not those of `skip`.
+template <int F> struct Filter {
+    static constexpr int kind = F;
+    Bits legal, skip;
+    __device__ __forceinline__ uint32_t out(int a, int len) const {
+        uint32_t o = F & 1 ? ~legal.field(a, len) : 0u;
+        if (F & 2) o |= skip.field(a, len);
+        return o;
+    }
+    __device__ __forceinline__ bool has(int a) const { return !((F & 1 && !legal.test(a)) || (F & 2 && skip.test(a))); }
+};
+
 // One turn: U chunks of a lane, loaded before the first is used.
-template <typename T, int W, int U, bool ENT, bool SKIP>
-__device__ __forceinline__ void lane_turn(LaneSum& z, const T* body, int i, Bits skip, int head, float c) {
+template <typename T, int W, int U, bool ENT, int F>
+__device__ __forceinline__ void lane_turn(LaneSum& z, const T* body, int i, Filter<F> f, int head, float c) {
     constexpr int E = Chunk<T>::E;
     Chunk<T> q[U];
 #pragma unroll
@@ -533,8 +581,8 @@ __device__ __forceinline__ void lane_turn(LaneSum& z, const T* body, int i, Bits
     float m = NEG_INF;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (SKIP) {
-            const uint32_t out = skip.field(head + (i + u * 32 * W) * E, E);
+        if (F) {
+            const uint32_t out = f.out(head + (i + u * 32 * W) * E, E);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 if ((out >> e) & 1) q[u].set(e, NEG_INF);
@@ -549,17 +597,17 @@ __device__ __forceinline__ void lane_turn(LaneSum& z, const T* body, int i, Bits
         for (int e = 0; e < E; ++e) lane_add<ENT>(z, q[u].get(e), ref, c);
 }
 
-template <typename T, int W, bool ENT, bool SKIP>
-__device__ __forceinline__ LaneSum pass_all(const T* x, Bits skip, int a, float c, int part) {
+template <typename T, int W, bool ENT, int F>
+__device__ __forceinline__ LaneSum pass_all(const T* x, Filter<F> f, int a, float c, int part) {
     constexpr int U = sizeof(T) == 4 ? 4 : 2;
     const Deal<T, W> deal(x, a, part);
     LaneSum z = {NEG_INF, 0.f, 0.f};
     const T* body = x + deal.head;
-    const float last = deal.end < a && !(SKIP && skip.test(deal.end)) ? to_f(x[deal.end]) : NEG_INF;
+    const float last = deal.end < a && f.has(deal.end) ? to_f(x[deal.end]) : NEG_INF;
     int i = deal.first;
-    for (; !SKIP && (i | 31) + (U - 1) * 32 * W < deal.chunks; i += U * 32 * W)  // while all lanes have U
-        lane_turn<T, W, U, ENT, false>(z, body, i, skip, 0, c);
-    for (; i < deal.chunks; i += 32 * W) lane_turn<T, W, 1, ENT, SKIP>(z, body, i, skip, deal.head, c);
+    for (; (i | 31) + (U - 1) * 32 * W < deal.chunks; i += U * 32 * W)  // while all lanes have U
+        lane_turn<T, W, U, ENT, F>(z, body, i, f, deal.head, c);
+    for (; i < deal.chunks; i += 32 * W) lane_turn<T, W, 1, ENT, F>(z, body, i, f, deal.head, c);
     lane_raise<ENT>(z, last, c);
     lane_add<ENT>(z, last, z.m == NEG_INF ? 0.f : z.m, c);
     return z;
@@ -567,23 +615,27 @@ __device__ __forceinline__ LaneSum pass_all(const T* x, Bits skip, int a, float 
 
 // The lanes' sums as the row's.  Where one action holds nearly all of the mass,
 // its lane goes over its own elements once more for the sum of the others.
-template <typename T, int W, bool ENT>
-__device__ __forceinline__ Sum whole_all(LaneSum z, const T* x, int a, float c, int part, Sum* sh) {
-    const float m = warp_max(z.m), d = (z.m - m) * c, f = m == NEG_INF ? 1.f : exp2_(d);
+template <typename T, int W, bool ENT, int F>
+__device__ __forceinline__ Sum whole_all(LaneSum z, const T* x, Filter<F> f, int a, float c, int part, Sum* sh) {
+    const float m = warp_max(z.m), d = (z.m - m) * c, w = m == NEG_INF ? 1.f : exp2_(d);
     const bool top = z.m == m && m > NEG_INF;
-    Sum s = {m, top ? 1.f : 0.f, top ? z.s - 1.f : f * z.s, ENT ? f * (z.t + z.s * fmaxf(d, -1e4f)) : 0.f};
+    Sum s = {m, top ? 1.f : 0.f, top ? z.s - 1.f : w * z.s, ENT ? w * (z.t + z.s * fmaxf(d, -1e4f)) : 0.f};
     Sum r = whole<W>(s, c, sh);
     if (r.n == 1.f && r.r < 0.015625f) {
         if (z.m == r.m) {
+            constexpr int E = Chunk<T>::E;
             const Deal<T, W> deal(x, a, part);
             float rest = 0.f;
+            auto add = [&](float v) { rest += v == r.m ? 0.f : exp2_((v - r.m) * c); };
             for (int i = deal.first; i < deal.chunks; i += 32 * W) {
                 Chunk<T> q;
-                q.load(x + deal.head + i * Chunk<T>::E);
+                q.load(x + deal.head + i * E);
+                const uint32_t out = F ? f.out(deal.head + i * E, E) : 0u;
 #pragma unroll
-                for (int e = 0; e < Chunk<T>::E; ++e) rest += q.get(e) == r.m ? 0.f : exp2_((q.get(e) - r.m) * c);
+                for (int e = 0; e < E; ++e)
+                    if (!(F && (out >> e) & 1)) add(q.get(e));
             }
-            if (deal.end < a && to_f(x[deal.end]) != r.m) rest += exp2_((to_f(x[deal.end]) - r.m) * c);
+            if (deal.end < a && f.has(deal.end)) add(to_f(x[deal.end]));
             s.r = rest;
         }
         if (W > 1) __syncthreads();
@@ -623,8 +675,9 @@ template <int W> __device__ __forceinline__ float kth_peak(const float (*peaks)[
 }
 
 // This lane's elements of `low` and more, into cand[0 .. limit).
-template <typename T, int W>
-__device__ __forceinline__ void list_from(float low, const T* x, int a, int part, uint64_t* cand, int limit, int* count) {
+template <typename T, int W, int F>
+__device__ __forceinline__ void list_from(float low, const T* x, Filter<F> f, int a, int part, uint64_t* cand, int limit,
+                                          int* count) {
     constexpr int E = Chunk<T>::E;
     const Deal<T, W> deal(x, a, part);
     auto keep = [&](int b) {
@@ -638,10 +691,11 @@ __device__ __forceinline__ void list_from(float low, const T* x, int a, int part
             uint32_t hit = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) hit |= q.get(e) >= low ? 1u << e : 0u;
+            if (F) hit &= ~f.out(deal.head + i * E, E);
             for (; hit; hit &= hit - 1) keep(deal.head + i * E + __ffs(hit) - 1);
         }
     }
-    if (deal.end < a && to_f(x[deal.end]) >= low) keep(deal.end);
+    if (deal.end < a && f.has(deal.end) && to_f(x[deal.end]) >= low) keep(deal.end);
 }
 
 __device__ __forceinline__ void top_of_list(Top& top, const uint64_t* cand, int n) {
@@ -656,15 +710,15 @@ __device__ __forceinline__ void top_of_list(Top& top, const uint64_t* cand, int 
 
 // Where too many reach the bound (equal or sorted logits): a warp's part, all
 // lanes' elements in turn.
-template <typename T, int W>
-__device__ __forceinline__ void top_of_part(Top& top, const T* x, int a, int part) {
+template <typename T, int W, int F>
+__device__ __forceinline__ void top_of_part(Top& top, const T* x, Filter<F> f, int a, int part) {
     constexpr int E = Chunk<T>::E;
     const Deal<T, W> deal(x, a, part);
     const int rounds = (deal.chunks + 32 * W - 1) / (32 * W) * E;
-    top.offer(deal.end < a ? to_f(x[deal.end]) : NEG_INF, deal.end);
+    top.offer(deal.end < a && f.has(deal.end) ? to_f(x[deal.end]) : NEG_INF, deal.end);
     for (int i = 0; i < rounds; ++i) {
         const int ch = deal.first + i / E * 32 * W, b = deal.head + ch * E + i % E;
-        top.offer(ch < deal.chunks ? to_f(x[b]) : NEG_INF, b);
+        top.offer(ch < deal.chunks && f.has(b) ? to_f(x[b]) : NEG_INF, b);
     }
 }
 
@@ -714,19 +768,15 @@ __device__ __forceinline__ void grad_sparse(const T* x, T* g, int first, int a, 
     }
 }
 
-// The same with every action legal.
-template <typename T, bool ENT>
+// A chunk with every action legal.  NEAR: the logits do not lie as the gradient does.
+template <typename T, bool ENT, bool NEAR>
 __device__ __forceinline__ void grad_dense(const T* x, T* g, int first, int a, const RowGrad& r, float inv_t) {
     constexpr int E = Chunk<T>::E;
     Chunk<T> q;
-    if (first >= 0 && first + E <= a) {
-        if (((intptr_t)(x + first) & 31) == 0) {
-            q.load(x + first);
-        } else {
-            q.fill(0);
-#pragma unroll
-            for (int e = 0; e < E; ++e) q.set(e, to_f(x[first + e]));
-        }
+    bool full = first >= 0 && first + E <= a;
+    if (NEAR) full = q.load_near(x, first, a);
+    else if (full) q.load(x + first);
+    if (full) {
 #pragma unroll
         for (int e = 0; e < E; ++e) q.set(e, grad_of<ENT>(q.get(e), r, r.c0, 0.f, inv_t));
         q.store(g + first);
@@ -752,7 +802,10 @@ __device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, con
     const int chunks = (a + e0 + E - 1) / E, per = (chunks + W - 1) / W;
     const int lo = part * per, hi = min(chunks, lo + per);
     if (MASK == SB_MASK_NONE) {
-        for (int ch = lo + lane; ch < hi; ch += 32) grad_dense<T, ENT>(x, g, ch * E - e0, a, r, inv_t);
+        if ((((intptr_t)x ^ (intptr_t)g) & 31) == 0)
+            for (int ch = lo + lane; ch < hi; ch += 32) grad_dense<T, ENT, false>(x, g, ch * E - e0, a, r, inv_t);
+        else
+            for (int ch = lo + lane; ch < hi; ch += 32) grad_dense<T, ENT, true>(x, g, ch * E - e0, a, r, inv_t);
     } else {
         uint32_t* list = reinterpret_cast<uint32_t*>(sh);
         T* xs = reinterpret_cast<T*>(sh + 4 * CHUNKS + lane * SLOT);
@@ -781,9 +834,12 @@ __device__ __forceinline__ int2 grad_row(const T* x, T* g, Bits bits, int a, con
                 for (int k = from + lane; k < to; k += 32)
                     if (!open(k, bits.field(k * E - e0, E))) zero.store(g + k * E - e0);
                 if (lane < count) grad_sparse<T, ENT>(x, g, first0, a, v0 >> 16, wide, q, r, inv_t, xs, gs);
-                for (int i = lane + 32; i < count; i += 32) {
-                    const uint32_t v = list[i];
-                    grad_sparse<T, ENT>(x, g, (int)(v & 0xffffu) * E - e0, a, v >> 16, false, q, r, inv_t, xs, gs);
+                if (lane + 32 < count) {  // at most CHUNKS = 64 are listed
+                    const uint32_t v = list[lane + 32];
+                    const int first = (int)(v & 0xffffu) * E - e0;
+                    const bool too = first >= 0 && first + E <= a && ((intptr_t)(x + first) & 31) == 0;
+                    if (too) q.load(x + first);
+                    grad_sparse<T, ENT>(x, g, first, a, v >> 16, too, q, r, inv_t, xs, gs);
                 }
                 __syncwarp();
                 count = 0;

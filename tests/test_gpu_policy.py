@@ -544,6 +544,46 @@ def test_distill_tail_when_everything_is_listed(kind):
     assert torch.isfinite(loss).all()
 
 
+@pytest.mark.parametrize("kind", ["none", "bool", "bits"])
+@pytest.mark.parametrize("a", [50, 600, 10000])
+@pytest.mark.parametrize("density", [0.05, 0.7])
+def test_distill_tail_with_a_near_certain_rest(a, density, kind):
+    """The listed actions hold nearly all of the student's mass, and one unlisted action nearly all of what is left."""
+    g = torch.Generator().manual_seed(a)
+    ok = torch.rand((6, a), generator=g) < density
+    ok[:, :4] = True
+    x = -12.0 + 0.1 * torch.randn((6, a), generator=g)
+    x[:, :3] = torch.tensor([9.0, 8.0, 10.0])
+    x[:, 3] = 5.0
+    ta = torch.tensor([[0, 1, 2]]).expand(6, 3).contiguous()
+    tl = torch.log(torch.tensor([[0.5, 0.2, 0.1]])).expand(6, 3).contiguous()
+    _check_distill(x, ok, ta, tl, kind, 1.0, True)
+
+
+@pytest.mark.parametrize("kind", ["none", "bool", "bits"])
+@pytest.mark.parametrize("a, density", [(60, 0.5), (700, 0.02), (700, 0.8), (10000, 0.8)])
+def test_confident_rows(a, density, kind):
+    """One action holds all but a little of the mass: its log-probability, the entropy and the gradient of the rest."""
+    g = torch.Generator().manual_seed(a)
+    ok = torch.rand((5, a), generator=g) < density
+    ok[:, 1] = True
+    x = torch.randn((5, a), generator=g)
+    x[:, 1] = torch.tensor([14.0, 20.0, 30.0, 60.0, 300.0])
+    _check_logprobs(x, ok, torch.ones(5, dtype=torch.int64), kind, top=3, t=1.0)
+
+
+def test_second_derivatives_are_refused():
+    from ataraxos_b200.policy import action_logprobs, distill_loss
+
+    x = torch.randn(4, 30, device=DEV, requires_grad=True)
+    act = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for y in (action_logprobs(x, act).logprob, action_logprobs(x, act, top=2).entropy,
+              distill_loss(x, act[:, None], torch.zeros(4, 1, device=DEV))):
+        first = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            first.square().sum().backward()
+
+
 def test_distill_of_itself_is_zero():
     from ataraxos_b200.policy import action_logprobs, distill_loss
 

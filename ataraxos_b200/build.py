@@ -29,11 +29,12 @@ DEPS = SOURCES + [CSRC / "sb_device.cuh", CSRC / "sb_error.h", CSRC / "sb_policy
 TORCH_LIB_PATH = LIB_DIR / "libstratego_b200_torch.so"
 TORCH_SOURCE = CSRC / "sb_torch.cpp"
 
-NVCC_FLAGS = [
+COMPILE_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
+NVCC_FLAGS = [*COMPILE_FLAGS, "-shared"]
 
 
 def nvcc() -> str:
@@ -56,8 +57,7 @@ def _compile(path: Path, extra: list[str], verbose: bool) -> None:
         cmds, objs = [], []
         for src in SOURCES:
             objs.append(str(Path(tmp) / f"{src.stem}.o"))
-            cmds.append([nvcc(), *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS[:-3], *extra, f"-I{INCLUDE}",
-                         "-Xcompiler", "-fPIC", "-c", "-o", objs[-1], str(src)])
+            cmds.append([nvcc(), *(["-Xptxas=-v"] if verbose else []), *COMPILE_FLAGS, *extra, f"-I{INCLUDE}", "-c", "-o", objs[-1], str(src)])
         lib = Path(tmp) / path.name
         if verbose:
             print("\n".join(" ".join(c) for c in cmds), flush=True)

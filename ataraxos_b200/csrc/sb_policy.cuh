@@ -861,8 +861,8 @@ inline int check_rows(const sb_logits* x, Rows* R) {
     if (x->dtype != SB_DTYPE_F32 && x->dtype != SB_DTYPE_BF16 && x->dtype != SB_DTYPE_F16)
         return fail(SB_E_ARG, "bad logits dtype %d", x->dtype);
     if (x->mask_kind < SB_MASK_NONE || x->mask_kind > SB_MASK_BITS) return fail(SB_E_ARG, "bad mask kind %d", x->mask_kind);
-    if (!(x->temperature > 0.f) || x->temperature == INFINITY || 1.f / x->temperature == INFINITY)
-        return fail(SB_E_ARG, "temperature must be finite and > 0");
+    if (!(x->temperature >= 1e-30f && x->temperature <= 1e30f))
+        return fail(SB_E_ARG, "temperature must be between 1e-30 and 1e30");
     if (x->row_stride < 0 || x->mask_stride < 0) return fail(SB_E_ARG, "negative row stride");
     if (x->n_rows == 0) return SB_OK;
     if (!x->logits || !aligned(x->logits, x->dtype == SB_DTYPE_F32 ? 4 : 2))

@@ -15,17 +15,19 @@ network's ``action_logprobs(..., top=k)``, or a search policy
 
 Both take the masks as the simulator writes them, uint8 / bool per action
 (``[..., 10000]`` or ``[..., 100, 100]``) or bit-packed (``[..., 1250]``), and
-any other number of actions up to 65,536.  A masked-out logit is never looked
+any other number of actions A up to 65,536 (bit-packed: ``ceil(A / 8)`` bytes; a
+mask of one byte for one action is that action's).  A masked-out logit is never looked
 at, so it may be anything, NaN included.  Sums and statistics are float32 for
 float32, bfloat16 and float16 logits alike; gradients are rounded once, to the
 logits' type.  A legal NaN or +inf makes its row's results NaN.
 
 Both launch on the current torch stream of the logits' device and can be
 captured into a CUDA graph, gradients included (as with any torch operator, no
-eager autograd graph of the same leaf tensor may be alive then).  The gradient is computed from the logits, the
-mask and the listed actions again: leave them unchanged until the backward
-pass has run (the masks and observations of ``step`` are overwritten by the
-next step; ``TrajectoryBuffer`` keeps them).
+eager autograd graph of the same leaf tensor may be alive then).  The gradient
+is computed from the logits, the mask and the listed actions again: leave them
+unchanged until the backward pass has run (the masks and observations of
+``step`` are overwritten by the next step; ``TrajectoryBuffer`` keeps them).
+The gradients have no derivatives of their own.
 """
 
 from __future__ import annotations

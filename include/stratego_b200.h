@@ -360,7 +360,7 @@ typedef struct sb_logits {
     int32_t n_actions;         /* 1 .. SB_POLICY_MAX_ACTIONS */
     int32_t dtype;             /* SB_DTYPE_F32 / BF16 / F16 */
     int32_t mask_kind;         /* SB_MASK_* */
-    float temperature;         /* finite, > 0 */
+    float temperature;         /* 1e-30 .. 1e30 */
 } sb_logits;
 
 /* Log-probabilities of given actions with entropy and top alternatives. */

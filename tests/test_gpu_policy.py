@@ -572,6 +572,30 @@ def test_confident_rows(a, density, kind):
     _check_logprobs(x, ok, torch.ones(5, dtype=torch.int64), kind, top=3, t=1.0)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("kind", ["none", "bool", "bits"])
+@pytest.mark.parametrize("a, k", [(100, 40), (900, 70), (10000, 200), (20000, 65)])
+def test_distill_entries_listed_again_far_apart(a, k, kind, tail):
+    """The same action in different groups of 32 entries, with different weights; entries left out in between."""
+    x, ok, g = _rows(5, a, torch.float32, 0.5 if a < 10000 else 0.02, seed=k)
+    ta, tl = _teacher(x, torch.ones_like(ok) if kind == "none" else ok, k, g, tail, 1.3)
+    ta[0, 33:37] = ta[0, 0:4]
+    ta[3, k - 1] = ta[3, 0]
+    ta[3, k // 2] = ta[3, 0]
+    ta[4, 5::7] = -1
+    if tail:
+        tl[:, 32:] -= 1.0                                # the weights stay below 1 in sum
+    _check_distill(x, ok, ta, tl, kind, 1.3, tail)
+
+
+@pytest.mark.parametrize("kind", ["bits", "bool", "none"])
+@pytest.mark.parametrize("dtype, density", [(torch.bfloat16, 0.5), (torch.float32, 0.02), (torch.float16, 1.0)])
+def test_batches_of_more_than_a_thousand_rows(dtype, density, kind):
+    """Where a gradient row is one warp's."""
+    x, ok, g = _rows(1300, 2600, dtype, density, seed=21)
+    _check_logprobs(x, ok, _actions(torch.ones_like(ok) if kind == "none" else ok, g), kind, top=0, t=1.0)
+
+
 def test_second_derivatives_are_refused():
     from ataraxos_b200.policy import action_logprobs, distill_loss
 

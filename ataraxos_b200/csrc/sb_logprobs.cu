@@ -7,6 +7,12 @@ namespace {
 
 // ---- forward: given actions, entropy, top alternatives -----------------------------
 
+// One pass over the row for (M, Z, H), the action's logit beside it, then the
+// outputs.  Masked rows are bound by the chain mask -> legal actions -> their
+// logits and by instructions (730 a row): 65,536 bf16 rows of 10,000 with bit
+// masks 60 us (144 MB, 2.4 TB/s), 4096 with u8 masks 12.2 us (45 MB, 3.7 TB/s).
+// Unmasked rows by latency and instructions: 2049 f32 rows of 9999 with top 8
+// 27.8 us (82 MB, 2.9 TB/s).
 template <typename T, int MASK, int W, bool TOP>
 __device__ __forceinline__ void logprobs_rows(const Rows& R, const sb_logprobs& o) {
     extern __shared__ uint4 dyn[];
@@ -118,6 +124,8 @@ __global__ void __launch_bounds__(WARPS * 32, 10) logprobs_top_kernel(const __gr
     logprobs_rows<T, MASK, 1, true>(R, o);
 }
 
+// The gradient's bytes bound it: 65,536 bf16 rows with bit masks 266 us
+// (1.46 GB, 5.5 TB/s; the zeros alone, without reading a mask, took 222 us).
 template <typename T, int MASK, int W>
 __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, sb_logprobs f, sb_logprobs_grad g) {
     extern __shared__ uint4 dyn[];

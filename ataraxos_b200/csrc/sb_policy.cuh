@@ -15,12 +15,13 @@
 // first, so large logits lose nothing).
 //
 // Layout of the work: a row belongs to one warp, or to the four warps of a
-// CTA where it is long (wide_forward, wide_backward).  That rule looks at the
-// shape and the types alone, so a row's bits do not depend on the batch it
-// comes in.  A legal mask is
-// staged in shared memory as one bit per action, and only the logits of set
-// bits are read: a position has some 30 legal moves of 10,000, so a row costs
-// its mask and 30 sectors instead of 20 or 40 KB.
+// CTA where it is long (wide_forward, wide_backward).  In the forward pass that
+// rule looks at the shape and the types alone, and a gradient's elements do not
+// depend on who computes them, so a row's bits do not depend on its batch.  A
+// legal mask is staged in shared memory as one bit per action, and only the
+// logits of set bits are read: a position has some 30 legal moves of 10,000, so
+// a row costs its mask and 30 sectors instead of 20 or 40 KB.  A row of which
+// over an eighth is legal is read whole.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -7,7 +7,7 @@ namespace {
 
 // ---- distillation ------------------------------------------------------------------------
 
-// Kept per row for the backward pass: (M, log Z), (Q, Q - q_r / p_r) and the
+// Kept per row for the backward pass: (M, log Z), (Q, log(q_r / p_r)) and the
 // teacher's own (maximum, log sum).
 
 // This lane's teacher entry of a round of 32: its action (-1 where it is left
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
             }
         }
         const float2 st = stats_of(s);
-        float loss = 0.f, total = 0.f, share = 0.f;
+        float loss = 0.f, total = 0.f, log_ratio = NEG_INF;
         float2 tst = make_float2(0.f, 0.f);
         bool more = false;  // a second pass is needed
         bool lead0 = false;  // entry e0 is its action's first
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
                 if (qr > 0.f && !more) {
                     const float lqr = log1pf(-total), lpr = log1pf(-sp);
                     loss += qr * (lqr - lpr);
-                    share = expf(lqr - lpr);
+                    log_ratio = lqr - lpr;
                     total += qr;
                 }
             }
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
                     const float qr = fmaxf(0.f, 1.f - total), lqr = log1pf(-total);
                     const float lpr = (sr.x - st.x) * R.inv_t + sr.y - st.y;
                     loss += qr * (lqr - lpr);
-                    share = expf(lqr - lpr);
+                    log_ratio = lqr - lpr;
                     total += qr;
                 }
             }
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
             if (d.row_stats) {
                 float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
                 o[0] = st;
-                o[1] = make_float2(total, total - share);
+                o[1] = make_float2(total, log_ratio);
                 o[2] = tst;
             }
         }
@@ -234,8 +234,9 @@ __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb
         }
         auto entry = [&](int k0) { return entry_of<T, MASK>(R, x, bits, load_raw(d, row, k0 + lane)); };
         const Entry e0 = entry_of<T, MASK>(R, x, bits, raw);
-        const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
-        const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, r, R.inv_t, work, W == 1 ? 0 : warp);
+        const RowGrad r = {st.x, st.y, 0.f, 0.f, w * co.x};  // of the listed actions
+        const int2 own = grad_row<T, MASK, W, false>(x, out, bits, R.a, rest_grad(st, co.x, co.y, w), R.inv_t, work,
+                                                   W == 1 ? 0 : warp);
         for (int k0 = 0; k0 < d.listed; k0 += 32) {
             const Entry e = k0 ? entry(k0) : e0;
             float q = e.a >= 0 ? expf((e.v - te.x) * tc - te.y) : 0.f;

@@ -787,6 +787,16 @@ __device__ __forceinline__ void grad_dense(const T* x, T* g, int first, int a, c
     }
 }
 
+// A distilled row's gradient off the listed actions, w (p Q - q_r p / p_r) / T,
+// from Q and the logarithm of q_r / p_r (-inf: no rest).  The ratio itself
+// leaves float32's range where the policy puts next to nothing on the rest, and
+// p with it; so a ratio above 1 goes into the exponent, and what is
+// exponentiated is log(q_r p / p_r) <= 0.
+__device__ __forceinline__ RowGrad rest_grad(float2 stats, float total, float log_ratio, float w) {
+    const float k = fmaxf(0.f, log_ratio);
+    return {stats.x, stats.y - k, w * (total * expf(-k) - expf(log_ratio - k)), 0.f, 0.f};
+}
+
 // Shared memory of a warp's gradient work: the list and two slots a lane.
 constexpr int GRAD_BYTES = 4 * CHUNKS + 2 * 32 * SLOT;
 

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(WARPS * 32, 10) small_distill_kernel(Rows R, i
             s.r = group_sum(s.r);
             tst = stats_of(s);
         }
-        float loss = 0.f, total = 0.f, share = 0.f;
+        float loss = 0.f, total = 0.f, log_ratio = NEG_INF;
         uint32_t listed = 0;  // bit i: the lane's action l + 8 i is listed
         for (int k = l; k < (d.listed + G - 1) / G * G; k += G) {
             float v;
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(WARPS * 32, 10) small_distill_kernel(Rows R, i
             if (qr > 0.f && (sp < 0.5f || s.m > NEG_INF)) {
                 const float lqr = log1pf(-total), lpr = sp < 0.5f ? log1pf(-sp) : (sr.x - st.x) * R.inv_t + sr.y - st.y;
                 loss += qr * (lqr - lpr);
-                share = expf(lqr - lpr);
+                log_ratio = lqr - lpr;
                 total += qr;
             }
         }
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(WARPS * 32, 10) small_distill_kernel(Rows R, i
             if (d.row_stats) {
                 float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
                 o[0] = st;
-                o[1] = make_float2(total, total - share);
+                o[1] = make_float2(total, log_ratio);
                 o[2] = tst;
             }
         }
@@ -352,15 +352,16 @@ __global__ void __launch_bounds__(WARPS * 32, 8) small_distill_backward_kernel(R
                 }
             }
         }
-        const RowGrad r = {st.x, st.y, w * co.y, 0.f, w * co.x};
+        const RowGrad r = {st.x, st.y, 0.f, 0.f, w * co.x}, rest = rest_grad(st, co.x, co.y, w);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int a = l + G * i;
             if (a < R.a) {
                 const bool on = (listed >> i) & 1;
                 const float e = on ? -w * wt[a] : 0.f;
+                const RowGrad s = {r.m, on ? r.logz : rest.logz, 0.f, 0.f, 0.f};
                 sh[q * R.a + a] =
-                    from_f<T>((p.ok >> i) & 1 ? grad_of<false>(p.v[i], r, on ? r.l0 : r.c0, e, R.inv_t) : 0.f);
+                    from_f<T>((p.ok >> i) & 1 ? grad_of<false>(p.v[i], s, on ? r.l0 : rest.c0, e, R.inv_t) : 0.f);
             }
         }
         store_rows(sh, grad + row0 * R.a, R.a, R.n - row0);

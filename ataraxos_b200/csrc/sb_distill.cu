@@ -182,10 +182,10 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
                     pass_masked<T, W, false, false, true>(rest, none, x, bits, skip, R.a, c, list, part);
                     rest = whole<W>(rest, c, sums);
                 }
-                if ((W == 1 || warp == 0) && rest.m > NEG_INF) {
-                    const float2 sr = stats_of(rest);
+                const float2 sr = stats_of(rest);
+                const float lpr = rest.m > NEG_INF ? (sr.x - st.x) * R.inv_t + sr.y - st.y : NEG_INF;
+                if ((W == 1 || warp == 0) && lpr > LOG_NO_MASS) {
                     const float qr = fmaxf(0.f, 1.f - total), lqr = log1pf(-total);
-                    const float lpr = (sr.x - st.x) * R.inv_t + sr.y - st.y;
                     loss += qr * (lqr - lpr);
                     log_ratio = lqr - lpr;
                     total += qr;

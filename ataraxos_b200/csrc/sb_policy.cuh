@@ -787,6 +787,12 @@ __device__ __forceinline__ void grad_dense(const T* x, T* g, int first, int a, c
     }
 }
 
+// A rest whose mass p_r the policy takes below e^-745, where 64-bit floats end,
+// counts as no rest: such actions are masked inside the logits (-1e9, the
+// type's lowest value), and what rounding leaves of a teacher that lists all
+// the others must not be set against them.
+constexpr float LOG_NO_MASS = -745.f;
+
 // A distilled row's gradient off the listed actions, w (p Q - q_r p / p_r) / T,
 // from Q and the logarithm of q_r / p_r (-inf: no rest).  The ratio itself
 // leaves float32's range where the policy puts next to nothing on the rest, and

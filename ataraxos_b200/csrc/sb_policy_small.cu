@@ -296,8 +296,11 @@ __global__ void __launch_bounds__(WARPS * 32, 10) small_distill_kernel(Rows R, i
             sp = group_sum(sp);
             const Sum s = sum_part<false>(p, rest, c);
             const float2 sr = stats_of(s);
-            if (qr > 0.f && (sp < 0.5f || s.m > NEG_INF)) {
-                const float lqr = log1pf(-total), lpr = sp < 0.5f ? log1pf(-sp) : (sr.x - st.x) * R.inv_t + sr.y - st.y;
+            const float lpr = sp < 0.5f          ? log1pf(-sp)
+                              : s.m > NEG_INF ? (sr.x - st.x) * R.inv_t + sr.y - st.y
+                                              : NEG_INF;
+            if (qr > 0.f && lpr > LOG_NO_MASS) {
+                const float lqr = log1pf(-total);
                 loss += qr * (lqr - lpr);
                 log_ratio = lqr - lpr;
                 total += qr;

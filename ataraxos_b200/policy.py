@@ -126,7 +126,10 @@ def distill_loss(
     ``tail=True``: ``teacher_logits`` are the teacher's log-probabilities at
     this temperature, as ``action_logprobs(..., top=K, temperature=...)`` gives
     them, and all legal actions that are not listed count as one entry: the
-    teacher's mass left over against the policy's own mass on them.
+    teacher's mass left over against the policy's own mass on them.  Where the
+    policy has no mass there (no such action, or less than ``e**-745``, as for
+    actions masked inside the logits by -inf, -1e9 or the type's lowest value)
+    what is left over is dropped.
 
     The gradient flows to ``logits`` only.  Multiply by ``temperature ** 2`` to
     keep its scale when mixing it with a loss at temperature 1.

@@ -398,7 +398,9 @@ int sb_action_logprobs_backward(const sb_logits *x, const sb_logprobs *fwd, cons
  *   tail = 0: q = softmax(teacher logits / temperature) over the entries left;
  *   tail = 1: the teacher logits are log-probabilities (at this temperature),
  *     q = exp of them, and the actions not listed count as one more entry of
- *     mass 1 - sum q against the policy's own mass on them. */
+ *     mass 1 - sum q against the policy's own mass on them.  Where that is 0
+ *     (no such action, or below e^-745: logits of -inf, -1e9 or the type's
+ *     lowest value) there is no such entry, and the mass left over is dropped. */
 typedef struct sb_distill {
     const void *teacher_actions; /* [n_rows,listed] signed integers; one listed twice counts twice */
     const void *teacher_logits;  /* [n_rows,listed] */

@@ -52,3 +52,26 @@ def test_rest_far_below_many_listed_actions(a, kind):
     tl[1, 35] = -7.0
     loss, grad = _check_distill(x, ok, ta, tl, kind, 1.0, True)
     assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("kind", ["none", "bool", "bits"])
+@pytest.mark.parametrize("a", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("spare", [0.0, 0.3])
+def test_rest_without_mass(spare, dtype, a, kind):
+    """Moves masked inside the logits (-1e9, the type's lowest value, -inf on places that the mask allows) and a teacher
+    that lists all real ones: what rounding (or ``spare``) leaves of its mass is not set against nothing."""
+    g = torch.Generator().manual_seed(a)
+    ok = torch.rand((4, a), generator=g) < 0.4
+    ok[:, :12] = True
+    low = torch.finfo(dtype).min
+    x = torch.randn((4, a), generator=g)
+    x[:, 12:] = torch.tensor([max(-1e9, low), low, -float("inf"), -2000.0])[:, None]
+    x = x.to(dtype)
+    real = torch.zeros_like(ok)
+    real[:, :12] = True
+    ta, tl = _teacher(x, real, 12, g, True, 1.0)
+    tl += torch.log1p(torch.tensor(-spare))
+    loss, grad = _check_distill(x, ok, ta, tl, kind, 1.0, True)
+    assert loss.abs().max().item() < 20 and torch.isfinite(grad).all()
+    assert not grad[:, 12:].any()

@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(WARPS * 32, 10) small_distill_kernel(Rows R, i
             }
         }
         if (live && l == 0) {
-            d.loss[row] = loss;
+            d.loss[row] = st.y != st.y ? NAN : loss;  // a spoiled row's, whatever is kept
             if (d.row_stats) {
                 float2* o = reinterpret_cast<float2*>(d.row_stats + 6 * row);
                 o[0] = st;

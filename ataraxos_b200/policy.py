@@ -19,7 +19,8 @@ any other number of actions A up to 65,536 (bit-packed: ``ceil(A / 8)`` bytes; a
 mask of one byte for one action is that action's).  A masked-out logit is never looked
 at, so it may be anything, NaN included.  Sums and statistics are float32 for
 float32, bfloat16 and float16 logits alike; gradients are rounded once, to the
-logits' type.  A legal NaN or +inf makes its row's results NaN.
+logits' type.  A legal NaN or +inf makes its row's results NaN (the
+log-probability of an action that has none, -1 or not legal, aside).
 
 Both launch on the current torch stream of the logits' device and can be
 captured into a CUDA graph, gradients included (as with any torch operator, no

@@ -7,6 +7,7 @@
 // The kernels stay behind the C ABI: bind() receives the addresses of its
 // entry points, so this file links against torch alone.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -58,12 +59,19 @@ int dtype_code(const Tensor& t) {
     }
 }
 
+// Forward mode: a dual tensor need not require grad, and an output without a
+// tangent would count as a constant.
+bool has_tangent(const Tensor& t) {
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+
 void check_logits(const Tensor& x, double temperature) {
     TORCH_CHECK(dtype_code(x) >= 0, "logits must be a float32, bfloat16 or float16 tensor");
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= SB_POLICY_MAX_ACTIONS,
                 "logits must be [..., A] with 1 <= A <= ", SB_POLICY_MAX_ACTIONS, ", got ", x.sizes());
     TORCH_CHECK(std::isfinite(temperature) && temperature >= 1e-30 && temperature <= 1e30,
                 "temperature must be between 1e-30 and 1e30, got ", temperature);
+    TORCH_CHECK(!has_tangent(x), "the policy operators have no forward-mode derivatives: pass the logits' primal");
 }
 
 // [..., W] as [R, W] with the elements of a row side by side: a view where the
@@ -344,6 +352,8 @@ Tensor distill_loss(const Tensor& logits, const Tensor& teacher_actions, const T
                 teacher_logits.sizes(), " on ", teacher_logits.device());
     TORCH_CHECK(!(at::GradMode::is_enabled() && teacher_logits.requires_grad()),
                 "distill_loss has no gradient for teacher_logits: detach them");
+    TORCH_CHECK(!has_tangent(teacher_logits),
+                "distill_loss has no forward-mode derivative for teacher_logits: pass their primal");
     const Mask m = mask_rows(mask, logits);
     check_cuda(logits);
     Tensor tl = teacher_logits.contiguous();

@@ -28,7 +28,8 @@ eager autograd graph of the same leaf tensor may be alive then).  The gradient
 is computed from the logits, the mask and the listed actions again: leave them
 unchanged until the backward pass has run (the masks and observations of
 ``step`` are overwritten by the next step; ``TrajectoryBuffer`` keeps them).
-The gradients have no derivatives of their own.
+The gradients have no derivatives of their own, and there are none in forward
+mode: a dual tensor is refused.
 """
 
 from __future__ import annotations

@@ -29,7 +29,10 @@ is computed from the logits, the mask and the listed actions again: leave them
 unchanged until the backward pass has run (the masks and observations of
 ``step`` are overwritten by the next step; ``TrajectoryBuffer`` keeps them).
 The gradients have no derivatives of their own, and there are none in forward
-mode: a dual tensor is refused.
+mode: a dual tensor is refused, and so is ``vmap``.  Fake tensors, traced graphs
+(``make_fx``) and ``torch.compile`` take a call as one opaque operator for each
+kernel; call an operator once before a compilation with ``fullgraph=True``, since
+the first call binds the library.
 """
 
 from __future__ import annotations

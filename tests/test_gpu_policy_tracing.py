@@ -1,0 +1,99 @@
+"""The policy operators in traced and compiled functions: the same bits as eager calls (no code is generated)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_gpu_policy import DEV, _actions, _pack, _rows, _teacher
+from torch.fx.experimental.proxy_tensor import make_fx
+
+pytestmark = pytest.mark.gpu
+
+
+def _operands(r=6, a=3000, seed=1, dtype=torch.float32):
+    x, ok, g = _rows(r, a, dtype, 0.02, seed=seed)
+    ta, tl = _teacher(x, ok, 8, g, True, 1.0)
+    return tuple(v.to(DEV) for v in (x, _actions(ok, g), ta, tl, _pack(ok)))
+
+
+def _values(x, act, ta, tl, bits):
+    from ataraxos_b200.policy import action_logprobs, distill_loss
+
+    r = action_logprobs(x, act, bits, top=3)
+    return r.logprob, r.entropy, r.top_logprob, r.top_action, distill_loss(x, ta, tl, bits, tail=True)
+
+
+def _both(x, *rest):
+    x = x.detach().requires_grad_()
+    v = _values(x, *rest)
+    some = v[3] >= 0
+    pull = v[0].sum() + 0.5 * v[1].sum() + torch.where(some, v[2], 0.0).sum() + v[4].sum()
+    return (*(t.detach() for t in v), torch.autograd.grad(pull, x)[0])
+
+
+def _same(got, want):
+    for p, q in zip(got, want, strict=True):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_traced_graph_launches_the_kernels(dtype):
+    """Forward and gradient recorded on one set of operands and run on others, laid out otherwise too."""
+    g = make_fx(_both)(*_operands(dtype=dtype))
+    names = [str(n.target) for n in g.graph.nodes if str(n.target).startswith("stratego_b200.")]
+    assert sorted(names) == sorted(f"stratego_b200.{n}.default" for n in (
+        "_action_logprobs", "_distill_loss", "_action_logprobs_backward", "_distill_loss_backward"))
+    other = _operands(seed=2, dtype=dtype)
+    want = _both(*other)
+    _same(g(*other), want)
+    spread = tuple(v.t().contiguous().t() if v.dim() == 2 else v.repeat_interleave(2)[::2] for v in other)
+    assert spread[0].stride(1) != 1 and spread[1].stride(0) == 2
+    _same(g(*spread), want)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_functions_keep_their_results(backend):
+    """torch.compile with static and then changing numbers of rows, forward and gradient."""
+    torch._dynamo.reset()
+
+    def loss(x, act, ta, tl, bits):
+        v = _values(x, act, ta, tl, bits)
+        return v[0].sum() + 0.5 * v[1].sum() + v[4].sum(), v[3]
+
+    fast = torch.compile(loss, backend=backend)
+    for r in (6, 6, 11, 4):
+        x, *rest = _operands(r, seed=r)
+        lx, ly = x.clone().requires_grad_(), x.clone().requires_grad_()
+        got, top = fast(lx, *rest)
+        want, ref = loss(ly, *rest)
+        got.backward()
+        want.backward()
+        _same((got, top, lx.grad), (want, ref, ly.grad))
+        with torch.no_grad():
+            _same(fast(x, *rest), loss(x, *rest))
+    torch._dynamo.reset()
+
+
+def test_one_graph_once_the_library_is_loaded():
+    torch._dynamo.reset()
+    args = _operands()
+    want = _values(*args)  # an eager call has bound the library
+    _same(torch.compile(_values, backend="aot_eager", fullgraph=True)(*args), want)
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("what", ["mask", "actions", "teacher", "gradient"])
+def test_rows_that_do_not_belong_together_are_refused(what):
+    """What a traced graph calls checks its operands before it launches."""
+    ops = torch.ops.stratego_b200
+    x, act, ta, tl, bits = _operands()
+    _values(x, act, ta, tl, bits)
+    loss, stats = ops._distill_loss(x, ta, tl, bits, 2, 1.0, True, True)
+    calls = {
+        "mask": lambda: ops._action_logprobs(x, act, bits[:5], 2, 0, 1.0, False),
+        "actions": lambda: ops._action_logprobs(x, act[:5], bits, 2, 0, 1.0, False),
+        "teacher": lambda: ops._distill_loss(x, ta, tl[:, :7], bits, 2, 1.0, True, False),
+        "gradient": lambda: ops._distill_loss_backward(x, ta, tl, bits, 2, stats, loss[:5], 1.0, True),
+    }
+    with pytest.raises(RuntimeError, match="do not match"):
+        calls[what]()

@@ -143,8 +143,11 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_backward_kernel(Rows R, s
         int mine = -1;
         float add = 0.f;
         if (g.g_top && lane < f.top) {
-            mine = (int)f.top_action[row * f.top + lane];
-            if (mine >= 0) add = g.g_top[row * f.top + lane];
+            const int64_t a = f.top_action[row * f.top + lane];
+            if (a >= 0 && a < R.a) {
+                mine = (int)a;
+                add = g.g_top[row * f.top + lane];
+            }
         }
         int64_t act = -1;
         float ga = 0.f;

@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8) small_logprobs_backward_kernel(
             float shares = 0.f;
             for (int k = l; live && k < f.top; k += G) {
                 const int64_t a = f.top_action[row * f.top + k];
-                if (a >= 0) {
+                if (a >= 0 && a < R.a) {
                     add[a] = g.g_top[row * f.top + k];
                     shares += add[a];
                 }

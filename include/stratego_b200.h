@@ -379,8 +379,9 @@ typedef struct sb_logprobs {
 int sb_action_logprobs(const sb_logits *x, const sb_logprobs *out, void *stream);
 
 /* Gradient with respect to the logits; x, actions, top, entropy, row_stats
- * and top_action as the forward call had or wrote them.  The gradients of the
- * outputs may be NULL (zero).  Every element of grad is written (0 where the
+ * and top_action as the forward call had or wrote them (an alternative outside
+ * 0 .. n_actions - 1 is left out).  The gradients of the outputs may be NULL
+ * (zero).  Every element of grad is written (0 where the
  * action is not legal). */
 typedef struct sb_logprobs_grad {
     const float *g_logprob;    /* element r at [r * g_logprob_stride] (stride 0 or 1) */

@@ -291,7 +291,7 @@ int sb_distill_loss(const sb_logits* x, const sb_distill* d, void* stream) {
     Rows R;
     int rc = check_rows(x, &R);
     if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
-    if (!d->loss) return fail(SB_E_ARG, "loss is NULL");
+    if (!d->loss || !aligned(d->loss, 4)) return fail(SB_E_ARG, "loss is NULL or not aligned to its type");
     if (R.a <= SMALL) return small_distill(x, *d, (cudaStream_t)stream);
     return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -312,7 +312,8 @@ int sb_distill_loss_backward(const sb_logits* x, const sb_distill* d, const floa
     int rc = check_rows(x, &R);
     if (rc != SB_OK || (rc = check_distill(x, d)) != SB_OK || x->n_rows == 0) return rc;
     if (!g_loss || !grad || !d->row_stats) return fail(SB_E_ARG, "g_loss, grad or row_stats is NULL");
-    if (!aligned(grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
+    if (!aligned(grad, x->dtype == SB_DTYPE_F32 ? 4 : 2) || !aligned(g_loss, 4))
+        return fail(SB_E_ARG, "grad or g_loss not aligned to its type");
     if (R.a <= SMALL) return small_distill_backward(x, *d, g_loss, g_loss_stride, grad, (cudaStream_t)stream);
     return dispatch(x, wide_backward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;

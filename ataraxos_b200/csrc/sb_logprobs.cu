@@ -202,7 +202,9 @@ int sb_action_logprobs(const sb_logits* x, const sb_logprobs* out, void* stream)
     if (!out->entropy || (out->actions != nullptr) != (out->logprob != nullptr))
         return fail(SB_E_ARG, "entropy is NULL, or actions and logprob disagree");
     if (out->top && (!out->top_action || !out->top_logprob)) return fail(SB_E_ARG, "top outputs are NULL");
-    if (out->row_stats && !aligned(out->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
+    if (!aligned(out->entropy, 4) || !aligned(out->logprob, 4) || !aligned(out->row_stats, 8) ||
+        (out->top && (!aligned(out->top_action, 8) || !aligned(out->top_logprob, 4))))
+        return fail(SB_E_ARG, "an output is not aligned to its type (row_stats: 8 bytes)");
     if (R.a <= SMALL) return small_logprobs(x, *out, (cudaStream_t)stream);
     return dispatch(x, wide_forward(x), [&](auto* t, auto mask, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -227,7 +229,9 @@ int sb_action_logprobs_backward(const sb_logits* x, const sb_logprobs* fwd, cons
     if (x->n_rows == 0) return SB_OK;
     if (!g->grad || !fwd->row_stats || !fwd->entropy) return fail(SB_E_ARG, "grad, row_stats or entropy is NULL");
     if (!aligned(g->grad, x->dtype == SB_DTYPE_F32 ? 4 : 2)) return fail(SB_E_ARG, "grad not aligned to its type");
-    if (!aligned(fwd->row_stats, 8)) return fail(SB_E_ARG, "row_stats not 8-byte aligned");
+    if (!aligned(fwd->row_stats, 8) || !aligned(fwd->entropy, 4) || !aligned(g->g_logprob, 4) ||
+        !aligned(g->g_entropy, 4) || (g->g_top && (!aligned(g->g_top, 4) || !aligned(fwd->top_action, 8))))
+        return fail(SB_E_ARG, "an operand is not aligned to its type (row_stats: 8 bytes)");
     if ((g->g_logprob && !fwd->actions) || (g->g_top && (!fwd->top || !fwd->top_action)))
         return fail(SB_E_ARG, "a gradient of an output that the forward call did not have");
     if (R.a <= SMALL) return small_logprobs_backward(x, *fwd, *g, (cudaStream_t)stream);

@@ -135,9 +135,13 @@ Mask mask_rows(const std::optional<Tensor>& given, const Tensor& logits) {
     return {as_rows(m), bytes ? SB_MASK_U8 : SB_MASK_BITS};
 }
 
-Tensor index_rows(const Tensor& t, c10::SymIntArrayRef shape, const char* what, const Tensor& logits) {
+void check_index(const Tensor& t, const char* what) {
     TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt || t.scalar_type() == at::kShort, what,
                 " must be an int16, int32 or int64 tensor");
+}
+
+Tensor index_rows(const Tensor& t, c10::SymIntArrayRef shape, const char* what, const Tensor& logits) {
+    check_index(t, what);
     TORCH_CHECK(t.sym_sizes() == shape, what, " must have shape ", shape, ", got ", t.sym_sizes());
     TORCH_CHECK(t.device() == logits.device(), what, " are on ", t.device(), ", the logits are on ", logits.device());
     return t.contiguous();
@@ -189,10 +193,18 @@ struct Rows {
         arg.mask_kind = (int32_t)kind;
         arg.temperature = (float)temperature;
     }
-    // `t`, one or `width` elements for each row, as the kernels read it.
+    // `t`, `width` elements for each row, as the kernels read it.
     Tensor beside(const Tensor& t, int64_t width, const char* what) const {
         TORCH_CHECK(t.device() == x.device() && t.numel() == x.size(0) * width, what, " do not match logits ", x.sizes());
         return t.contiguous();
+    }
+    Tensor beside(const Tensor& t, int64_t width, at::ScalarType type, const char* what) const {
+        TORCH_CHECK(t.scalar_type() == type, what, " must be ", type, ", got ", t.scalar_type());
+        return beside(t, width, what);
+    }
+    Tensor indices(const Tensor& t, int64_t width, const char* what) const {
+        check_index(t, what);
+        return beside(t, width, what);
     }
 };
 
@@ -246,7 +258,7 @@ variable_list logprobs_rows(const Tensor& logits, const std::optional<Tensor>& a
     Tensor act;
     sb_logprobs arg = {};
     if (actions.has_value()) {
-        act = rows.beside(*actions, 1, "actions");
+        act = rows.indices(*actions, 1, "actions");
         arg.actions = act.data_ptr();
         arg.action_bytes = (int32_t)act.element_size();
     }
@@ -281,17 +293,18 @@ Tensor logprobs_rows_backward(const Tensor& logits, const std::optional<Tensor>&
     Tensor act, top, gt;
     sb_logprobs f = {};
     if (actions.has_value()) {
-        act = rows.beside(*actions, 1, "actions");
+        act = rows.indices(*actions, 1, "actions");
         f.actions = act.data_ptr();
         f.action_bytes = (int32_t)act.element_size();
     }
     if (top_action.has_value()) {
         f.top = (int32_t)top_action->size(-1);
-        top = rows.beside(*top_action, f.top, "alternatives");
+        top = rows.beside(*top_action, f.top, at::kLong, "alternatives");
         f.top_action = ptr<int64_t>(top);
         if (g_top.has_value()) gt = rows.beside(*g_top, f.top, "gradients").to(at::kFloat);
     }
-    const Tensor h = rows.beside(entropy, 1, "entropies"), stats = rows.beside(row_stats, 2, "statistics");
+    const Tensor h = rows.beside(entropy, 1, at::kFloat, "entropies"),
+                 stats = rows.beside(row_stats, 2, at::kFloat, "statistics");
     f.entropy = ptr<float>(h);
     f.row_stats = ptr<float>(stats);
     const RowGrad ge(rows, g_entropy.value_or(Tensor())), gl(rows, g_logprob.value_or(Tensor()));
@@ -370,7 +383,7 @@ struct Teacher {
     sb_distill arg = {};
     Teacher(const Rows& rows, const Tensor& actions, const Tensor& logits, bool tail) {
         TORCH_CHECK(actions.dim() == 2 && dtype_code(logits) >= 0, "the teacher must be rows of actions and floats");
-        ta = rows.beside(actions, actions.size(1), "teacher_actions");
+        ta = rows.indices(actions, actions.size(1), "teacher_actions");
         tl = rows.beside(logits, actions.size(1), "teacher_logits");
         arg.teacher_actions = ta.data_ptr();
         arg.teacher_logits = tl.data_ptr();
@@ -417,7 +430,7 @@ Tensor distill_rows_backward(const Tensor& logits, const Tensor& teacher_actions
     const Rows rows(logits, mask, kind, temperature);
     Teacher t(rows, teacher_actions, teacher_logits, tail);
     Tensor grad = at::empty(rows.x.sizes(), rows.x.options().requires_grad(false));
-    const Tensor stats = rows.beside(row_stats, 6, "statistics");
+    const Tensor stats = rows.beside(row_stats, 6, at::kFloat, "statistics");
     t.arg.row_stats = ptr<float>(stats);
     const RowGrad g(rows, g_loss);
     if (rows.arg.n_rows)

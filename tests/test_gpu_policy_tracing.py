@@ -82,6 +82,27 @@ def test_one_graph_once_the_library_is_loaded():
     torch._dynamo.reset()
 
 
+@pytest.mark.parametrize("what", ["actions", "alternatives", "statistics", "teacher"])
+def test_rows_of_another_type_are_refused(what):
+    ops = torch.ops.stratego_b200
+    x, act, ta, tl, bits = _operands()
+    _values(x, act, ta, tl, bits)
+    ent, _, _, best, stats = ops._action_logprobs(x, act, bits, 2, 3, 1.0, True)
+
+    def back(best=best, stats=stats):
+        return ops._action_logprobs_backward(x, act, bits, 2, best, ent, stats, ent, None, None, 1.0)
+
+    back()
+    calls = {
+        "actions": lambda: ops._action_logprobs(x, act.double(), bits, 2, 0, 1.0, False),
+        "alternatives": lambda: back(best=best.int()),
+        "statistics": lambda: back(stats=stats.half()),
+        "teacher": lambda: ops._distill_loss(x, ta.double(), tl, bits, 2, 1.0, True, False),
+    }
+    with pytest.raises(RuntimeError, match="must be"):
+        calls[what]()
+
+
 @pytest.mark.parametrize("what", ["mask", "actions", "teacher", "gradient"])
 def test_rows_that_do_not_belong_together_are_refused(what):
     """What a traced graph calls checks its operands before it launches."""

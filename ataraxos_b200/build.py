@@ -28,6 +28,7 @@ DEPS = SOURCES + [CSRC / "sb_device.cuh", CSRC / "sb_error.h", CSRC / "sb_policy
 # the policy operators as torch operators: C++ against torch's headers, no CUDA code
 TORCH_LIB_PATH = LIB_DIR / "libstratego_b200_torch.so"
 TORCH_SOURCE = CSRC / "sb_torch.cpp"
+TORCH_STAMP = LIB_DIR / "libstratego_b200_torch.built_with"  # the torch that they were compiled against
 
 COMPILE_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -57,7 +58,8 @@ def _compile(path: Path, extra: list[str], verbose: bool) -> None:
         cmds, objs = [], []
         for src in SOURCES:
             objs.append(str(Path(tmp) / f"{src.stem}.o"))
-            cmds.append([nvcc(), *(["-Xptxas=-v"] if verbose else []), *COMPILE_FLAGS, *extra, f"-I{INCLUDE}", "-c", "-o", objs[-1], str(src)])
+            cmds.append([nvcc(), *(["-Xptxas=-v"] if verbose else []), *COMPILE_FLAGS, *extra, f"-I{INCLUDE}",
+                         "-c", "-o", objs[-1], str(src)])
         lib = Path(tmp) / path.name
         if verbose:
             print("\n".join(" ".join(c) for c in cmds), flush=True)
@@ -66,6 +68,18 @@ def _compile(path: Path, extra: list[str], verbose: bool) -> None:
                 done.check_returncode()
         subprocess.run([nvcc(), *NVCC_FLAGS, "-o", str(lib), *objs], check=True)
         os.replace(lib, path)
+
+
+def _torch_in_use() -> str:
+    import torch
+
+    return f"{torch.__version__} {Path(torch.__file__).resolve().parent} cxx11_abi={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
+def torch_up_to_date() -> bool:
+    """The torch operators are newer than their source and were compiled against this torch's headers and ABI."""
+    return (up_to_date(TORCH_LIB_PATH, [TORCH_SOURCE, INCLUDE / "stratego_b200.h"])
+            and TORCH_STAMP.exists() and TORCH_STAMP.read_text() == _torch_in_use())
 
 
 def _compile_torch(verbose: bool) -> None:
@@ -81,8 +95,10 @@ def _compile_torch(verbose: bool) -> None:
            "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)
+    TORCH_STAMP.unlink(missing_ok=True)  # a build that stops half way is built again
     subprocess.run(cmd, check=True)
     os.replace(tmp, TORCH_LIB_PATH)
+    TORCH_STAMP.write_text(_torch_in_use())
 
 
 def build(force: bool = False, verbose: bool = False, debug: bool = True) -> Path:
@@ -91,7 +107,7 @@ def build(force: bool = False, verbose: bool = False, debug: bool = True) -> Pat
         _compile(LIB_PATH, [], verbose)
     if debug and (force or not up_to_date(DEBUG_LIB_PATH)):
         _compile(DEBUG_LIB_PATH, ["-DSB_DEBUG_BOUNDS"], verbose)
-    if force or not up_to_date(TORCH_LIB_PATH, [TORCH_SOURCE, INCLUDE / "stratego_b200.h"]):
+    if force or not torch_up_to_date():
         _compile_torch(verbose)
     return LIB_PATH
 

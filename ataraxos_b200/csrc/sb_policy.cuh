@@ -17,8 +17,11 @@
 // Layout of the work: a row belongs to one warp, or to the four warps of a
 // CTA where it is long (wide_forward, wide_backward).  In the forward pass that
 // rule looks at the shape and the types alone, and a gradient's elements do not
-// depend on who computes them, so a row's bits do not depend on its batch.  A
-// legal mask is staged in shared memory as one bit per action, and only the
+// depend on who computes them.  So a row's bits do not depend on its batch nor
+// on where it lies, but for rows that are read whole (no mask, or over an eighth
+// legal, with more than SMALL actions): those are dealt to the lanes by sectors
+// of memory, and the order of their sums goes with the row's address modulo 32
+// bytes.  A legal mask is staged in shared memory as one bit per action, and only the
 // logits of set bits are read: a position has some 30 legal moves of 10,000, so
 // a row costs its mask and 30 sectors instead of 20 or 40 KB.  A row of which
 // over an eighth is legal is read whole.
@@ -441,8 +444,8 @@ struct Top {
 // a position's 30 legal moves lie in some 20 of 313 mask words: the words that
 // are not 0 (by ballots), then the actions of 32 such words, a lane each.  The
 // actions come out in ascending order and are dealt to the lanes in turn, so
-// the sums' order, and with it every bit of the result, is the same for any
-// kind of mask and wherever its rows lie.  SKIP leaves out the actions of
+// the sums' order, and with it every bit of a listed row's result, is the same
+// for any kind of mask and wherever its rows lie.  SKIP leaves out the actions of
 // `skip`.  Returns how many actions were taken, or -1, none taken, for a row of
 // one warp that is better read whole (pass_all): over half of its first words
 // hold a legal action, and over an eighth of their actions are legal.
@@ -939,9 +942,9 @@ inline bool wide_backward(const sb_logits* x) {
     return row_bytes(x) > 65536 || (row_bytes(x) > 4096 && x->n_rows < 8 * (int64_t)sms);
 }
 
-// Rows of up to SMALL actions: sb_policy_small.cu.
 }  // namespace
 
+// Rows of up to SMALL actions: sb_policy_small.cu.
 constexpr int SMALL = 128;
 int small_logprobs(const sb_logits* x, const sb_logprobs& o, cudaStream_t st);
 int small_logprobs_backward(const sb_logits* x, const sb_logprobs& f, const sb_logprobs_grad& g, cudaStream_t st);

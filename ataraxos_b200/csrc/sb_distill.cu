@@ -38,8 +38,8 @@ __device__ __forceinline__ Entry entry_of(const Rows& R, const T* x, Bits bits, 
 }
 
 // Loss (32,768 bf16 rows, bit masks, 32 listed, tail: 49 us; 4096 unmasked f16
-// rows 22.6 us, 82 MB at 3.6 TB/s): one pass for the row's (M, Z), then the teacher's entries by one warp.
-// With the tail, the unlisted actions' own mass p_r is 1 - sum p while that
+// rows 22.6 us, 82 MB at 3.6 TB/s): one pass for the row's (M, Z), then the
+// teacher's entries by one warp.  With the tail, the unlisted actions' own mass p_r is 1 - sum p while that
 // keeps its digits (sum p < 1/2), nothing where every legal action is listed,
 // and otherwise summed by a second pass that leaves the listed ones out.
 template <typename T, int MASK, int W, bool TAIL>
@@ -208,6 +208,9 @@ __global__ void __launch_bounds__(WARPS * 32) distill_kernel(Rows R, sb_distill 
 
 // Every row as p (Q - q_r / p_r), then the listed actions' own values over it.
 // Bound by the gradient's bytes: 32,768 bf16 rows 140 us (0.74 GB, 5.3 TB/s).
+// Above 32 listed every group of 32 walks all entries for repeats, which grows
+// with the square: 4096 bf16 rows under bit masks, forward and back together, 28
+// us at 32 listed, 37 at 64, 61 at 128, 513 at 512 (unmasked: 52, 74, 164, 1870).
 template <typename T, int MASK, int W>
 __global__ void __launch_bounds__(WARPS * 32) distill_backward_kernel(Rows R, sb_distill d, const float* g_loss,
                                                                       int64_t g_stride, T* grad) {

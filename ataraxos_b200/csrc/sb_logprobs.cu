@@ -116,8 +116,16 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(const __grid_const
 }
 
 // Masked rows with alternatives, a warp each: held to 48 registers, for the
-// sort takes 72 otherwise and the loads' latency wants the warps (16,384 rows,
-// 20 alternatives: 34.8 -> 26.6 us).
+// sort takes up to 72 otherwise and the loads' latency wants the warps.  All but
+// the 16-bit types under bit masks spill some of them (u8 masks have ten 16-byte
+// loads in flight), and still gain in large batches.  Without -> with the cap, 20
+// alternatives of 30 legal actions of 10,000, in us:
+//   rows                64          4096          16,384
+//   f32, u8         6.3 ->  7.8   18.9 -> 18.5   54.8 -> 52.9
+//   f32, bits       5.6 ->  6.1   10.7 ->  9.0   38.1 -> 29.7
+//   bf16 / f16, u8  6.6 ->  7.8   19.6 -> 17.8   56.9 -> 51.5
+//   bf16 / f16, bits 5.6 -> 5.8    8.0 ->  8.3   29.5 -> 26.7
+// Half of 10,000 legal, 16,384 rows: 204 -> 206 (bf16, bits) to 354 -> 307 (f32, u8).
 template <typename T, int MASK>
 __global__ void __launch_bounds__(WARPS * 32, 10) logprobs_top_kernel(const __grid_constant__ Rows R,
                                                                      const __grid_constant__ sb_logprobs o) {

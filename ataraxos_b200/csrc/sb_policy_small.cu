@@ -8,8 +8,10 @@
 // offset; the lanes of a row read neighbouring elements.  A gradient is put
 // together in shared memory and stored as the contiguous block that four rows
 // are.  The kernels are bound by their instructions (200,003 rows of 100 f16
-// logits: 91 a row forward in 29 us, 175 back in 39 us, against 6 us of bytes), so the actions of a lane are a constant, and by latency: the CTAs
-// per SM of their launch bounds were the fastest of 6 to 12.
+// logits: log-probabilities 91 a row forward in 29 us, 175 back in 39 us,
+// against 7 and 13 us of bytes; distillation of 16 listed with tail 56 and 65 us
+// against 12 and 19), so the actions of a lane are a constant, and by latency:
+// the CTAs per SM of their launch bounds were the fastest of 6 to 12.
 #include "sb_policy.cuh"
 
 namespace sb {

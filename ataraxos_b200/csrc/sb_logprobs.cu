@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(WARPS * 32) logprobs_kernel(const __grid_const
 }
 
 // Masked rows with alternatives, a warp each: held to 48 registers, for the
-// sort takes up to 72 otherwise and the loads' latency wants the warps.  All but
+// they take 64 to 96 otherwise and the loads' latency wants the warps.  All but
 // the 16-bit types under bit masks spill some of them (u8 masks have ten 16-byte
 // loads in flight), and still gain in large batches.  Without -> with the cap, 20
 // alternatives of 30 legal actions of 10,000, in us:

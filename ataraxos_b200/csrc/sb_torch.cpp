@@ -19,6 +19,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -531,6 +532,12 @@ TORCH_LIBRARY_IMPL(stratego_b200, CUDA, m) {
     m.impl("_action_logprobs_backward", &logprobs_rows_backward);
     m.impl("_distill_loss", &distill_rows);
     m.impl("_distill_loss_backward", &distill_rows_backward);
+}
+
+// A graph that was traced without gradients calls these with logits that require some: its backward pass raises.
+TORCH_LIBRARY_IMPL(stratego_b200, Autograd, m) {
+    for (const char* name : {"_action_logprobs", "_action_logprobs_backward", "_distill_loss", "_distill_loss_backward"})
+        m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }
 
 TORCH_LIBRARY_IMPL(stratego_b200, Meta, m) {

@@ -51,6 +51,39 @@ def test_a_traced_graph_launches_the_kernels(dtype):
     _same(g(*spread), want)
 
 
+def test_a_graph_traced_without_gradients_has_none():
+    """Run on logits that require grad, its values are right and its backward pass raises."""
+    args = _operands()
+    g = make_fx(_values)(*args)
+    x = args[0].clone().requires_grad_()
+    got = g(x, *args[1:])
+    _same(got, _values(*args))
+    assert not got[3].requires_grad
+    for v in (got[0], got[4]):
+        with pytest.raises(RuntimeError, match="not implemented"):
+            v.sum().backward()
+
+
+@pytest.mark.parametrize("public", ["action_logprobs", "distill_loss"])
+def test_torch_s_own_checks_of_an_operator(public):
+    """Schema, autograd registration, fake tensors and compilation with dynamic sizes, public and on rows."""
+    x, act, ta, tl, bits = _operands()
+    _values(x, act, ta, tl, bits)
+    ops = torch.ops.stratego_b200
+    lx = x.clone().requires_grad_()
+    if public == "action_logprobs":
+        out = ops._action_logprobs(x, act, bits, 2, 3, 1.0, True)
+        torch.library.opcheck(ops.action_logprobs.default, (lx, act, bits, 3, 1.0))
+        torch.library.opcheck(ops._action_logprobs.default, (x, act, bits, 2, 3, 1.0, True))
+        torch.library.opcheck(ops._action_logprobs_backward.default,
+                              (x, act, bits, 2, out[3], out[0], out[4], out[0], out[1], out[2], 1.0))
+    else:
+        loss, stats = ops._distill_loss(x, ta, tl, bits, 2, 1.0, True, True)
+        torch.library.opcheck(ops.distill_loss.default, (lx, ta, tl, bits, 1.0, True))
+        torch.library.opcheck(ops._distill_loss.default, (x, ta, tl, bits, 2, 1.0, True, True))
+        torch.library.opcheck(ops._distill_loss_backward.default, (x, ta, tl, bits, 2, stats, loss, 1.0, True))
+
+
 @pytest.mark.parametrize("backend", ["eager", "aot_eager"])
 def test_compiled_functions_keep_their_results(backend):
     """torch.compile with static and then changing numbers of rows, forward and gradient."""

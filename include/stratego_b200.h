@@ -371,7 +371,7 @@ typedef struct sb_logprobs {
     float *logprob;            /* [n_rows]: 0 where the action is -1 (none), -inf where it is not
                                   legal; may be NULL when actions is */
     float *entropy;            /* [n_rows]: 0 for a row without a legal action */
-    float *row_stats;          /* [n_rows,2] kept for the backward pass (may be NULL) */
+    float *row_stats;          /* [n_rows,2], 8-byte aligned, kept for the backward pass (may be NULL) */
     int64_t *top_action;       /* [n_rows,top] most likely first, ties to the lower action; -1
                                   past the last action of non-zero probability */
     float *top_logprob;        /* [n_rows,top], -inf there */
@@ -410,7 +410,7 @@ typedef struct sb_distill {
     int32_t listed;              /* 1 .. SB_POLICY_MAX_TEACHER */
     int32_t tail;                /* 0 or 1 */
     float *loss;                 /* [n_rows] */
-    float *row_stats;            /* [n_rows,6] kept for the backward pass (may be NULL) */
+    float *row_stats;            /* [n_rows,6], 8-byte aligned, kept for the backward pass (may be NULL) */
 } sb_distill;
 int sb_distill_loss(const sb_logits *x, const sb_distill *d, void *stream);
 /* Gradient with respect to the student's logits; g_loss element r at

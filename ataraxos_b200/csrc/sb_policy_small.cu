@@ -11,7 +11,9 @@
 // logits: log-probabilities 91 a row forward in 29 us, 175 back in 39 us,
 // against 7 and 13 us of bytes; distillation of 16 listed with tail 56 and 65 us
 // against 12 and 19), so the actions of a lane are a constant, and by latency:
-// the CTAs per SM of their launch bounds were the fastest of 6 to 12.
+// the CTAs per SM of their launch bounds were the fastest of 6 to 12, although the
+// forward kernels of 13 and 16 actions a lane spill some registers for them (48 to
+// 148 bytes read back in distillation, 40 in log-probabilities of 16).
 #include "sb_policy.cuh"
 
 namespace sb {
